@@ -27,6 +27,7 @@ EXPORTS = [
     "gcpnet_wg_reduce", "gcpnet_wg_reduce_multi", "gcpnet_dropout", "gcpnet_adam_step", "gcpnet_adam_step_dev", "gcpnet_copy2d_multi", "gcpnet_axpy_clamp_backward", "gcpnet_nms_edge_features", "gcpnet_nms_node_features", "gcpnet_radius_graph", "gcpnet_radius_graph_first", "gcpnet_activation", "gcpnet_frame_gate_forward", "gcpnet_frame_gate_backward",
     "gcpnet_frame_gate_bwd_parts", "gcpnet_node_scalarize", "gcpnet_orientations",
     "gcpnet_gcp2_weight_grads", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_stream_wait_stream", "gcpnet_wg_pack_multi",
+    "gcpnet_grad_norm_partials", "gcpnet_grad_norm", "gcpnet_adamw_begin", "gcpnet_adamw_step",
 ]
 
 
@@ -78,6 +79,15 @@ class Copy2dJob(C.Structure):
 
 class AdamTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("n", C.c_int64)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p),
+                ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("step", C.c_void_p), ("n", C.c_int64), ("ordinal", C.c_uint32),
+                ("vec", C.c_int)]
+
+
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 
 
 class WgBwdPlan(C.Structure):
@@ -156,6 +166,7 @@ def load():
     P = C.POINTER
     lib.gcpnet_abi_version.restype = i32
     lib.gcpnet_gcp2_pack_floats.restype = i64
+    lib.gcpnet_grad_norm_partials.restype = i64
     lib.gcpnet_gcp2_pack_floats.argtypes = [i32] * 6
     lib.gcpnet_gcp2_forward_lds_bytes.restype = i64
     lib.gcpnet_gcp2_forward_lds_bytes.argtypes = [i32] * 6
@@ -231,10 +242,15 @@ def load():
     lib.gcpnet_node_scalarize.argtypes = [i32, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp]
     lib.gcpnet_radius_graph.argtypes = [i32, vp, vp, vp, vp, i32, i32, i32, C.c_double, i32, vp, vp, vp]
     lib.gcpnet_radius_graph_first.argtypes = [i32, vp, vp, vp, vp, i32, i32, i32, C.c_double, i32, vp, vp, vp]
+    f64, AW = C.c_double, P(AdamWTensor)
+    lib.gcpnet_grad_norm_partials.argtypes = [i32, AW]
+    lib.gcpnet_grad_norm.argtypes = [i32, AW, i32, vp, vp]
+    lib.gcpnet_adamw_begin.argtypes = [i32, AW, f64, f64, f64, vp, vp, i64, f32, vp, vp]
+    lib.gcpnet_adamw_step.argtypes = [i32, AW, i32, i32, f64, f64, f64, f64, f64, vp, vp, C.c_uint32, vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("gcpnet_gcp2_pack_floats", "gcpnet_layernorm_bwd_scratch_floats", "gcpnet_gcp2_forward_lds_bytes",
-                        "gcpnet_wg_pack_floats", "gcpnet_tb_floats", "gcpnet_tb_sign_words", "gcpnet_gcp2_weight_grads_workspace"):
+                        "gcpnet_wg_pack_floats", "gcpnet_tb_floats", "gcpnet_tb_sign_words", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_grad_norm_partials"):
             fn.restype = i32
     if lib.gcpnet_abi_version() != 4:
         raise GcpnetHipError("libgcpnet_hip.so ABI version mismatch")

@@ -4,12 +4,12 @@ of them in one HIP launch per 96 tensors (gcpnet_adam_step) instead of several l
 from __future__ import annotations
 
 import ctypes as C
-from typing import Iterable
+from typing import Iterable, Optional
 
 import torch
 
 from . import _lib, ops
-from ._lib import AdamTensor, check
+from ._lib import AdamTensor, AdamWTensor, check
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -140,3 +140,226 @@ class FusedAdam(torch.optim.Optimizer):
         check(lib.gcpnet_adam_step(len(items), arr, float(group["lr"]), float(b1), float(b2), float(group["eps"]),
                                    float(group["weight_decay"]), int(step), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
               "adam_step")
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW(params, lr, betas, eps, weight_decay) semantics (decoupled weight decay, amsgrad=False, maximize=False) over all
+    tensors of a group in a few HIP launches, for fp32 and bf16 parameters on the GPU.
+
+    state_bits (32 or 8, per group): the moments `exp_avg`, `exp_avg_sq` in fp32, or as float8_e4m3fn codes with a power-of-two scale for
+    every 256 elements (`exp_avg_scale`, `exp_avg_sq_scale`): 2 bytes of state per element instead of 8.  exp_avg is rounded to nearest,
+    exp_avg_sq stochastically (unbiased; to nearest it would freeze), with a hash of (seed, position of the parameter, step, element):
+    the same run gives the same bits.  bf16 parameters keep an fp32 `master` copy in the state; a parameter whose value is not the
+    rounding of its master copy (loaded or edited since) is taken as it is.
+
+    max_grad_norm: every step scales the gradients (not their tensors: `p.grad` stays as it is) by min(1, max_grad_norm / (norm + 1e-6)) of
+    the norm over all groups, which `grad_norm` holds afterwards, on the device.
+
+    Nothing of a step depends on a host value that changes: `step` is a device tensor per parameter, and step() may be captured into a
+    hipGraph (GraphedStep(step_fn, optimizer=...)) once an eager step has created the state; lr, betas, eps and weight_decay are frozen
+    into a capture.  With state_bits=32 and fp32 parameters, state_dicts interchange with torch.optim.AdamW."""
+
+    def __init__(self, params: Iterable, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32, max_grad_norm: Optional[float] = None, seed: int = 0):
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed))
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            self._check_group(g)
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_options(g):
+        if isinstance(g["lr"], torch.Tensor):
+            raise TypeError("FusedAdamW: lr is a number (a tensor would be read back in every step)")
+        if not g["lr"] >= 0 or not g["eps"] >= 0 or not g["weight_decay"] >= 0:
+            raise ValueError("FusedAdamW: lr, eps and weight_decay must not be negative")
+        if not all(0 <= b < 1 for b in g["betas"]):
+            raise ValueError(f"FusedAdamW: betas must lie in [0, 1), got {g['betas']}")
+        if g["state_bits"] not in (8, 32):
+            raise ValueError(f"FusedAdamW: state_bits is 8 or 32, got {g['state_bits']}")
+
+    @classmethod
+    def _check_group(cls, g):
+        cls._check_options(g)
+        for p in g["params"]:
+            if p.dtype not in (torch.float32, torch.bfloat16):
+                raise TypeError(f"FusedAdamW: fp32 and bf16 parameters only, got {p.dtype}")
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.setdefault("max_grad_norm", None)
+        self.__dict__.setdefault("grad_norm", None)
+
+    def load_state_dict(self, state_dict):
+        """torch's loader converts every state tensor to its parameter's type: here the moments, scales and master copies keep theirs.
+        Moments of another kind (fp32 for a group with 8 bits, or the reverse) are refused."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for g in self.param_groups:  # (state of groups written by torch.optim.AdamW has no such keys)
+            g.setdefault("state_bits", self.defaults["state_bits"])
+            g.setdefault("seed", self.defaults["seed"])
+        mine = [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]
+        for i, (p, bits) in zip(saved, mine):
+            st = state_dict["state"].get(i)
+            if not st:
+                continue
+            new = {}
+            for key, v in st.items():
+                if key == "step":
+                    new[key] = torch.as_tensor(v).detach().to(device=p.device, dtype=torch.float32).reshape(()).clone()
+                elif key == "master" or key in ("exp_avg", "exp_avg_sq"):
+                    new[key] = torch.empty_like(p, dtype=v.dtype, memory_format=torch.preserve_format).copy_(v) if v.shape == p.shape else v
+                else:
+                    new[key] = v.detach().to(p.device).clone() if torch.is_tensor(v) else v
+            if p.dtype == torch.bfloat16 and bits == 32:  # (torch keeps the moments of bf16 parameters in bf16)
+                for key in ("exp_avg", "exp_avg_sq"):
+                    new[key] = new[key].float() if new[key].dtype == torch.bfloat16 else new[key]
+            if p.dtype == torch.bfloat16 and "master" not in new:
+                new["master"] = p.detach().float()
+            self._check_state(p, new, bits)
+            self.state[p] = new
+
+    @staticmethod
+    def _check_state(p, st, bits):
+        blocks = -(-p.numel() // 256)
+        want = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32}
+        if bits == 8:
+            want = {"exp_avg": torch.float8_e4m3fn, "exp_avg_sq": torch.float8_e4m3fn, "exp_avg_scale": None, "exp_avg_sq_scale": None}
+        if p.dtype == torch.bfloat16:
+            want["master"] = torch.float32
+        for key, dtype in want.items():
+            t = st.get(key)
+            if t is None or not torch.is_tensor(t) or t.device != p.device or t.dtype != (dtype or torch.float32):
+                raise _lib.GcpnetHipError(f"FusedAdamW: state {key!r} is missing, on another device or of another type than state_bits={bits} needs")
+            if dtype is None:
+                if t.numel() != blocks or not t.is_contiguous():
+                    raise _lib.GcpnetHipError(f"FusedAdamW: state {key!r} must hold {blocks} contiguous scales")
+            elif t.shape != p.shape or (t.stride() != p.stride() and not (t.is_contiguous() and p.is_contiguous())):
+                raise _lib.GcpnetHipError(f"FusedAdamW: state {key!r} must have its parameter's shape and strides")
+        step = st.get("step")
+        if not torch.is_tensor(step) or step.device != p.device or step.dtype != torch.float32 or step.numel() != 1:
+            raise _lib.GcpnetHipError("FusedAdamW: state 'step' must be one fp32 value on the parameter's device")
+
+    @staticmethod
+    def _new_state(p, bits):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: run at least one eager step before capturing (state is created there)")
+        st = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
+        dtype = torch.float32 if bits == 32 else torch.float8_e4m3fn
+        for key in ("exp_avg", "exp_avg_sq"):
+            # (zeros of one-byte codes through their bytes)
+            st[key] = torch.empty_like(p, dtype=dtype, memory_format=torch.preserve_format)
+            (st[key] if bits == 32 else st[key].view(torch.uint8)).zero_()
+            if bits == 8:
+                st[key + "_scale"] = torch.ones(-(-p.numel() // 256), dtype=torch.float32, device=p.device)
+        if p.dtype == torch.bfloat16:
+            st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+        return st
+
+    @staticmethod
+    def _dense(t) -> bool:
+        """Every element of the tensor's span once: elements in memory order are the tensor's."""
+        if t.is_contiguous():
+            return True
+        want = 1
+        for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+            if stride != want:
+                return False
+            want *= size
+        return True
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lib = _lib.load()
+        batches = {}  # (device, group, type) -> [(param, grad, state, ordinal)]
+        ordinal = 0
+        for gi, group in enumerate(self.param_groups):
+            self._check_options(group)
+            for p in group["params"]:
+                g = p.grad
+                ordinal += 1
+                if g is None:
+                    continue
+                if not p.is_cuda:
+                    raise _lib.GcpnetHipError("FusedAdamW: parameters on the GPU only (gcpnet_amd has no CPU path)")
+                if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+                    raise _lib.GcpnetHipError("FusedAdamW: a gradient must be dense and have its parameter's type, shape and device")
+                batches.setdefault((p.device.index, gi, p.dtype), []).append((p, g, ordinal - 1))
+        devices = {}
+        for (dev, gi, dtype), items in batches.items():
+            with torch.cuda.device(dev):
+                devices.setdefault(dev, []).append((gi, dtype, *self._table(items, self.param_groups[gi]["state_bits"])))
+        if len(devices) > 1 and self.max_grad_norm is not None:
+            raise _lib.GcpnetHipError("FusedAdamW: max_grad_norm with parameters on several devices is not supported")
+        for dev, parts in devices.items():
+            with torch.cuda.device(dev):
+                self._step_device(lib, dev, parts)
+        if batches:
+            touched = [p for items in batches.values() for p, _, _ in items]
+            torch.autograd.graph.increment_version(touched)  # (written through raw pointers: autograd's and the packs' caches must notice)
+            ops.invalidate_packs()
+        return loss
+
+    def _table(self, items, bits):
+        arr = (AdamWTensor * len(items))()
+        keep = []
+        for t, (p, g, ordinal) in zip(arr, items):
+            st = self.state[p]
+            if not self._dense(p):
+                raise _lib.GcpnetHipError("FusedAdamW: a parameter must fill its memory (a permuted tensor does, a slice of one does not)")
+            if "exp_avg" not in st:
+                st.update(self._new_state(p, bits))
+            else:
+                self._check_state(p, st, bits)
+            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+            keep.append(g)
+            t.param, t.grad, t.n, t.ordinal = p.data_ptr(), g.data_ptr(), p.numel(), ordinal
+            t.exp_avg, t.exp_avg_sq, t.step = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["step"].data_ptr()
+            if bits == 8:
+                t.exp_avg_scale, t.exp_avg_sq_scale = st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()
+            if p.dtype == torch.bfloat16:
+                t.master = st["master"].data_ptr()
+        return arr, keep
+
+    def _step_device(self, lib, dev, parts):
+        stream, where = ops._stream(), torch.device("cuda", dev)
+        types = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
+        total = sum(len(arr) for _, _, arr, _ in parts)
+        corr = torch.empty(2 * total, dtype=torch.float32, device=where)
+        clip = partials = None
+        count = 0
+        if self.max_grad_norm is not None:
+            counts = [int(lib.gcpnet_grad_norm_partials(len(arr), arr)) for _, _, arr, _ in parts]
+            count = sum(counts)
+            partials = torch.empty(max(count, 1), dtype=torch.float32, device=where)
+            clip = torch.empty(2, dtype=torch.float32, device=where)
+            at = 0
+            for (_, dtype, arr, _), c in zip(parts, counts):
+                check(lib.gcpnet_grad_norm(len(arr), arr, types[dtype], partials.data_ptr() + 4 * at, stream), "grad_norm")
+                at += c
+            self.grad_norm = clip[0]
+        at = 0
+        for k, (gi, dtype, arr, _) in enumerate(parts):
+            group = self.param_groups[gi]
+            (b1, b2), lr, here = group["betas"], float(group["lr"]), corr.data_ptr() + 8 * at
+            at += len(arr)
+            first = clip is not None and k == 0
+            check(lib.gcpnet_adamw_begin(len(arr), arr, lr, float(b1), float(b2), here, partials.data_ptr() if first else None, count,
+                                         float(self.max_grad_norm or 0.0), clip.data_ptr() if first else None, stream), "adamw_begin")
+            check(lib.gcpnet_adamw_step(len(arr), arr, types[dtype], int(group["state_bits"]), lr, float(b1), float(b2), float(group["eps"]),
+                                        float(group["weight_decay"]), here, None if clip is None else clip.data_ptr(),
+                                        int(group["seed"]) & 0xFFFFFFFF, stream), "adamw_step")

@@ -567,6 +567,40 @@ int gcpnet_adam_step(int n, const gcp_adam_tensor_t* tensors, float lr, float be
 int gcpnet_adam_step_dev(int n, const gcp_adam_tensor_t* tensors, float lr, float beta1, float beta2, float eps, float weight_decay,
                          int64_t* step_dev, void* stream);
 
+/* ---- AdamW over many tensors (decoupled weight decay; fp32 or bf16 parameters; moments in fp32, or in 8 bits: e4m3 codes with a
+ * power-of-two scale for every 256 elements in memory order).  A step is gcpnet_grad_norm (only when clipping), gcpnet_adamw_begin,
+ * gcpnet_adamw_step, on one stream; step counts, corrections and the clipping coefficient stay in device memory, so the three may be
+ * captured into a hipGraph.  bf16 parameters have an fp32 `master` copy; a parameter that is not the rounding of its master copy (it
+ * was written by somebody else) is taken as it is.  `ordinal`, the seed, the step count and an element's index decide the stochastic
+ * rounding of exp_avg_sq, so `ordinal` should differ between the tensors of a step.  `vec` is set by the library. */
+enum { GCP_TYPE_F32 = 0, GCP_TYPE_BF16 = 1, GCP_TYPE_F16 = 2 };
+typedef struct {
+    void* param;
+    const void* grad;
+    void* exp_avg;           /* fp32 [n] or e4m3 [n] */
+    void* exp_avg_sq;
+    float* exp_avg_scale;    /* [ceil(n / 256)]: 8 bits only */
+    float* exp_avg_sq_scale;
+    float* master;           /* [n]: bf16 only */
+    float* step;             /* steps taken so far, advanced by gcpnet_adamw_begin */
+    int64_t n;
+    uint32_t ordinal;
+    int vec;
+} gcp_adamw_tensor_t;
+#define GCP_ADAMW_MAX_TENSORS 44 /* per launch (any number per call) */
+#define GCP_ADAMW_MAX_BEGIN 448
+#define GCP_ADAMW_MAX_NORM 200
+/* floats that gcpnet_grad_norm writes: sums of squares over 16384 elements each */
+int64_t gcpnet_grad_norm_partials(int n, const gcp_adamw_tensor_t* tensors);
+int gcpnet_grad_norm(int n, const gcp_adamw_tensor_t* tensors, int type, float* partials, void* stream);
+/* step += 1 and corrections[2 k], [2 k + 1] = lr / (1 - beta1^step), sqrt(1 - beta2^step) for every tensor; with `partials` also
+ * clip[0], clip[1] = norm, min(1, max_norm / (norm + 1e-6)) */
+int gcpnet_adamw_begin(int n, const gcp_adamw_tensor_t* tensors, double lr, double beta1, double beta2, float* corrections,
+                       const float* partials, int64_t n_partials, float max_norm, float* clip, void* stream);
+int gcpnet_adamw_step(int n, const gcp_adamw_tensor_t* tensors, int type, int state_bits, double lr, double beta1, double beta2,
+                      double eps, double weight_decay, const float* corrections, const float* clip /* or NULL */, uint32_t seed,
+                      void* stream);
+
 /* ---- input side ---------------------------------------------------------------------------------
  * NMS featuriser, src/datamodules/components/nms_dataset.py:23-61 + helper.py:16-59:
  *   e_out [E, n_attr + n_rbf] = [edge_attr | RBF(|x_row - x_col|; mu = linspace(0, d_max, n_rbf), sigma = d_max / n_rbf)],
