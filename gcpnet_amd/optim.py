@@ -142,6 +142,29 @@ class FusedAdam(torch.optim.Optimizer):
               "adam_step")
 
 
+class _Part:
+    """The tensors of one parameter group that share a device and a type, as the launches take them."""
+
+    def __init__(self, device, dtype, items, bits):
+        self.device, self.dtype = device, dtype
+        self.type = _lib.TYPE_F32 if dtype == torch.float32 else _lib.TYPE_BF16
+        self.params = [p for p, _, _, _ in items]
+        self.arr = (AdamWTensor * len(items))()
+        self.known, self.copies = [], []
+        for t, (p, g, st, ordinal) in zip(self.arr, items):
+            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+                self.copies.append(g)  # (alive until the launches are enqueued)
+            t.param, t.grad, t.n, t.ordinal = p.data_ptr(), g.data_ptr(), p.numel(), ordinal
+            t.exp_avg, t.exp_avg_sq, t.step = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["step"].data_ptr()
+            if bits == 8:
+                t.exp_avg_scale, t.exp_avg_sq_scale = st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()
+            if dtype == torch.bfloat16:
+                t.master = st["master"].data_ptr()
+            # (a permuted parameter never matches: its table is built anew every step)
+            self.known.append((p, p.data_ptr() if p.is_contiguous() else None, p.numel(), tuple(map(id, st.values())), tuple(st.values())))
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW(params, lr, betas, eps, weight_decay) semantics (decoupled weight decay, amsgrad=False, maximize=False) over all
     tensors of a group in a few HIP launches, for fp32 and bf16 parameters on the GPU.
@@ -166,6 +189,7 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed))
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None
+        self._parts = {}
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -198,11 +222,16 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
+        self._parts = {}
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
 
     def load_state_dict(self, state_dict):
         """torch's loader converts every state tensor to its parameter's type: here the moments, scales and master copies keep theirs.
         Moments of another kind (fp32 for a group with 8 bits, or the reverse) are refused."""
         super().load_state_dict(state_dict)
+        self._parts = {}
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for g in self.param_groups:  # (state of groups written by torch.optim.AdamW has no such keys)
             g.setdefault("state_bits", self.defaults["state_bits"])
@@ -284,82 +313,94 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         lib = _lib.load()
-        batches = {}  # (device, group, type) -> [(param, grad, state, ordinal)]
-        ordinal = 0
+        devices, touched, ordinal = {}, [], 0  # device index -> [(group, _Part)]
         for gi, group in enumerate(self.param_groups):
             self._check_options(group)
-            for p in group["params"]:
-                g = p.grad
-                ordinal += 1
-                if g is None:
-                    continue
-                if not p.is_cuda:
-                    raise _lib.GcpnetHipError("FusedAdamW: parameters on the GPU only (gcpnet_amd has no CPU path)")
-                if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
-                    raise _lib.GcpnetHipError("FusedAdamW: a gradient must be dense and have its parameter's type, shape and device")
-                batches.setdefault((p.device.index, gi, p.dtype), []).append((p, g, ordinal - 1))
-        devices = {}
-        for (dev, gi, dtype), items in batches.items():
-            with torch.cuda.device(dev):
-                devices.setdefault(dev, []).append((gi, dtype, *self._table(items, self.param_groups[gi]["state_bits"])))
+            parts = self._parts.get(gi)
+            if parts is None or parts[0] != (ordinal, group["state_bits"]) or not self._refresh(parts[1], group["params"]):
+                parts = self._parts[gi] = ((ordinal, group["state_bits"]), self._build(group, ordinal))
+            ordinal += len(group["params"])
+            for part in parts[1]:
+                devices.setdefault(part.device, []).append((group, part))
+                touched += part.params
         if len(devices) > 1 and self.max_grad_norm is not None:
             raise _lib.GcpnetHipError("FusedAdamW: max_grad_norm with parameters on several devices is not supported")
         for dev, parts in devices.items():
             with torch.cuda.device(dev):
                 self._step_device(lib, dev, parts)
-        if batches:
-            touched = [p for items in batches.values() for p, _, _ in items]
+        if touched:
             torch.autograd.graph.increment_version(touched)  # (written through raw pointers: autograd's and the packs' caches must notice)
             ops.invalidate_packs()
+        for _, parts in self._parts.values():
+            for part in parts:
+                part.copies.clear()
         return loss
 
-    def _table(self, items, bits):
-        arr = (AdamWTensor * len(items))()
-        keep = []
-        for t, (p, g, ordinal) in zip(arr, items):
-            st = self.state[p]
+    def _build(self, group, ordinal):
+        """The launch tables of one group: every tensor looked at in full.  They hold what the optimizer owns (state addresses, sizes)
+        from step to step; parameters and gradients are looked up anew in each (`_refresh`)."""
+        parts = {}
+        bits = group["state_bits"]
+        for k, p in enumerate(group["params"]):
+            g = p.grad
+            if g is None:
+                continue
+            if not p.is_cuda:
+                raise _lib.GcpnetHipError("FusedAdamW: parameters on the GPU only (gcpnet_amd has no CPU path)")
+            if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+                raise _lib.GcpnetHipError("FusedAdamW: a gradient must be dense and have its parameter's type, shape and device")
+            if p.dtype not in (torch.float32, torch.bfloat16):
+                raise TypeError(f"FusedAdamW: fp32 and bf16 parameters only, got {p.dtype}")
             if not self._dense(p):
                 raise _lib.GcpnetHipError("FusedAdamW: a parameter must fill its memory (a permuted tensor does, a slice of one does not)")
-            if "exp_avg" not in st:
-                st.update(self._new_state(p, bits))
-            else:
-                self._check_state(p, st, bits)
-            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
-                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-            keep.append(g)
-            t.param, t.grad, t.n, t.ordinal = p.data_ptr(), g.data_ptr(), p.numel(), ordinal
-            t.exp_avg, t.exp_avg_sq, t.step = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["step"].data_ptr()
-            if bits == 8:
-                t.exp_avg_scale, t.exp_avg_sq_scale = st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()
-            if p.dtype == torch.bfloat16:
-                t.master = st["master"].data_ptr()
-        return arr, keep
+            st = self.state[p]
+            with torch.cuda.device(p.device):
+                if "exp_avg" not in st:
+                    st.update(self._new_state(p, bits))
+                else:
+                    self._check_state(p, st, bits)
+                parts.setdefault((p.device.index, p.dtype), []).append((p, g, st, ordinal + k))
+        return [_Part(dev, dtype, items, bits) for (dev, dtype), items in parts.items()]
+
+    def _refresh(self, parts, params) -> bool:
+        """Whether the same parameters take part with the same state as when `parts` were built; puts this step's gradients in."""
+        live = [id(p) for p in params if p.grad is not None]
+        if sorted(live) != sorted(id(p) for part in parts for p in part.params):
+            return False
+        state = self.state
+        for part in parts:
+            arr, dtype = part.arr, part.dtype
+            for k, (p, address, n, ids, _) in enumerate(part.known):
+                g = p.grad
+                if (g is None or not g.is_contiguous() or g.dtype is not dtype or g.numel() != n or p.data_ptr() != address
+                        or tuple(map(id, state[p].values())) != ids):
+                    return False
+                arr[k].grad = g.data_ptr()
+        return True
 
     def _step_device(self, lib, dev, parts):
         stream, where = ops._stream(), torch.device("cuda", dev)
-        types = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
-        total = sum(len(arr) for _, _, arr, _ in parts)
-        corr = torch.empty(2 * total, dtype=torch.float32, device=where)
+        corr = torch.empty(2 * sum(len(part.arr) for _, part in parts), dtype=torch.float32, device=where)
         clip = partials = None
         count = 0
         if self.max_grad_norm is not None:
-            counts = [int(lib.gcpnet_grad_norm_partials(len(arr), arr)) for _, _, arr, _ in parts]
+            counts = [int(lib.gcpnet_grad_norm_partials(len(part.arr), part.arr)) for _, part in parts]
             count = sum(counts)
             partials = torch.empty(max(count, 1), dtype=torch.float32, device=where)
             clip = torch.empty(2, dtype=torch.float32, device=where)
             at = 0
-            for (_, dtype, arr, _), c in zip(parts, counts):
-                check(lib.gcpnet_grad_norm(len(arr), arr, types[dtype], partials.data_ptr() + 4 * at, stream), "grad_norm")
+            for (_, part), c in zip(parts, counts):
+                check(lib.gcpnet_grad_norm(len(part.arr), part.arr, part.type, partials.data_ptr() + 4 * at, stream), "grad_norm")
                 at += c
             self.grad_norm = clip[0]
         at = 0
-        for k, (gi, dtype, arr, _) in enumerate(parts):
-            group = self.param_groups[gi]
+        for k, (group, part) in enumerate(parts):
+            arr = part.arr
             (b1, b2), lr, here = group["betas"], float(group["lr"]), corr.data_ptr() + 8 * at
             at += len(arr)
             first = clip is not None and k == 0
             check(lib.gcpnet_adamw_begin(len(arr), arr, lr, float(b1), float(b2), here, partials.data_ptr() if first else None, count,
                                          float(self.max_grad_norm or 0.0), clip.data_ptr() if first else None, stream), "adamw_begin")
-            check(lib.gcpnet_adamw_step(len(arr), arr, types[dtype], int(group["state_bits"]), lr, float(b1), float(b2), float(group["eps"]),
+            check(lib.gcpnet_adamw_step(len(arr), arr, part.type, int(group["state_bits"]), lr, float(b1), float(b2), float(group["eps"]),
                                         float(group["weight_decay"]), here, None if clip is None else clip.data_ptr(),
                                         int(group["seed"]) & 0xFFFFFFFF, stream), "adamw_step")
