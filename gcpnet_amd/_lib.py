@@ -28,6 +28,7 @@ EXPORTS = [
     "gcpnet_frame_gate_bwd_parts", "gcpnet_node_scalarize", "gcpnet_orientations",
     "gcpnet_gcp2_weight_grads", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_stream_wait_stream", "gcpnet_wg_pack_multi",
     "gcpnet_grad_norm_partials", "gcpnet_grad_norm", "gcpnet_adamw_begin", "gcpnet_adamw_step",
+    "gcpnet_block_norm_forward", "gcpnet_block_norm_backward", "gcpnet_block_norm_backward_scratch",
 ]
 
 
@@ -88,6 +89,16 @@ class AdamWTensor(C.Structure):
 
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+
+
+NORM = {None: 0, "layer": 1, "rms": 2}
+
+
+class BlockNorm(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("d", C.c_int), ("type", C.c_int), ("param_type", C.c_int), ("x", C.c_void_p), ("y", C.c_void_p),
+                ("gate", C.c_void_p), ("x_ld", C.c_int64), ("y_ld", C.c_int64), ("gate_ld", C.c_int64), ("post_w", C.c_void_p),
+                ("post_b", C.c_void_p), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p), ("post", C.c_int), ("pre", C.c_int), ("act", C.c_int),
+                ("scale", C.c_float), ("slope", C.c_float), ("eps", C.c_float)]
 
 
 class WgBwdPlan(C.Structure):
@@ -247,10 +258,15 @@ def load():
     lib.gcpnet_grad_norm.argtypes = [i32, AW, i32, vp, vp]
     lib.gcpnet_adamw_begin.argtypes = [i32, AW, f64, f64, f64, vp, vp, i64, f32, vp, vp]
     lib.gcpnet_adamw_step.argtypes = [i32, AW, i32, i32, f64, f64, f64, f64, f64, vp, vp, C.c_uint32, vp]
+    lib.gcpnet_block_norm_forward.argtypes = [P(BlockNorm), vp, vp, vp, vp]
+    lib.gcpnet_block_norm_backward.argtypes = [P(BlockNorm)] + [vp] * 13
+    lib.gcpnet_block_norm_backward_scratch.argtypes = [i64, i32]
+    lib.gcpnet_block_norm_backward_scratch.restype = i64
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("gcpnet_gcp2_pack_floats", "gcpnet_layernorm_bwd_scratch_floats", "gcpnet_gcp2_forward_lds_bytes",
-                        "gcpnet_wg_pack_floats", "gcpnet_tb_floats", "gcpnet_tb_sign_words", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_grad_norm_partials"):
+                        "gcpnet_wg_pack_floats", "gcpnet_tb_floats", "gcpnet_tb_sign_words", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_grad_norm_partials",
+                        "gcpnet_block_norm_backward_scratch"):
             fn.restype = i32
     if lib.gcpnet_abi_version() != 4:
         raise GcpnetHipError("libgcpnet_hip.so ABI version mismatch")

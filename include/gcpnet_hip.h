@@ -33,6 +33,9 @@ extern "C" {
 /* activation codes: models/__init__.py:42-57 (get_nonlinearity) */
 enum { GCP_ACT_NONE = 0, GCP_ACT_RELU = 1, GCP_ACT_LEAKYRELU = 2, GCP_ACT_SELU = 3, GCP_ACT_SILU = 4, GCP_ACT_SIGMOID = 5 };
 
+/* element types of the operators that take more than fp32 */
+enum { GCP_TYPE_F32 = 0, GCP_TYPE_BF16 = 1, GCP_TYPE_F16 = 2 };
+
 /* vector-gating mode of a GCP2 block: components/gcpnet.py:369-389 */
 enum { GCP_VMODE_NONE = 0, GCP_VMODE_SCALAR_GATE = 1 /* vector_gate */, GCP_VMODE_SELF_GATE = 2 /* sigma(norm) */ };
 
@@ -573,7 +576,6 @@ int gcpnet_adam_step_dev(int n, const gcp_adam_tensor_t* tensors, float lr, floa
  * captured into a hipGraph.  bf16 parameters have an fp32 `master` copy; a parameter that is not the rounding of its master copy (it
  * was written by somebody else) is taken as it is.  `ordinal`, the seed, the step count and an element's index decide the stochastic
  * rounding of exp_avg_sq, so `ordinal` should differ between the tensors of a step.  `vec` is set by the library. */
-enum { GCP_TYPE_F32 = 0, GCP_TYPE_BF16 = 1, GCP_TYPE_F16 = 2 };
 typedef struct {
     void* param;
     const void* grad;
@@ -600,6 +602,30 @@ int gcpnet_adamw_begin(int n, const gcp_adamw_tensor_t* tensors, double lr, doub
 int gcpnet_adamw_step(int n, const gcp_adamw_tensor_t* tensors, int type, int state_bits, double lr, double beta1, double beta2,
                       double eps, double weight_decay, const float* corrections, const float* clip /* or NULL */, uint32_t seed,
                       void* stream);
+
+/* ---- norms before and after a residual block with its gate and residual scale (fp32, bf16 or fp16 rows; everything in between in fp32):
+ *   u = post(y);  s = x + scale * act(gate) * u;  h = pre(s)
+ * over `rows` rows of `d` <= 16384 elements with unit column stride and row strides x_ld, y_ld, gate_ld (gate_ld 0: one value per channel).
+ * y NULL: s = x (no gate, no post).  Parameters [d] of param_type: fp32 or `type`; NULL weight = 1, NULL bias = 0.  Outputs are
+ * contiguous; s may be NULL, h is needed with pre.  stats [rows, 4] (16-byte aligned) is written for the backward, or NULL. */
+enum { GCP_NORM_NONE = 0, GCP_NORM_LAYER = 1, GCP_NORM_RMS = 2 };
+typedef struct {
+    int64_t rows;
+    int d, type, param_type;
+    const void *x, *y, *gate;
+    int64_t x_ld, y_ld, gate_ld;
+    const void *post_w, *post_b, *pre_w, *pre_b;
+    int post, pre, act;
+    float scale, slope, eps;
+} gcp_block_norm_t;
+int gcpnet_block_norm_forward(const gcp_block_norm_t* n, void* s, void* h, float* stats, void* stream);
+/* s: the forward's output s with row stride x_ld (the forward's x itself where y was NULL); ds, dh contiguous or NULL (= 0); outputs contiguous,
+ * each may be NULL; dgate is [rows, d], or [d] with gate_ld 0.  Column sums are formed in a fixed order.  scratch:
+ * gcpnet_block_norm_backward_scratch(rows, d) floats. */
+int64_t gcpnet_block_norm_backward_scratch(int64_t rows, int d);
+int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const void* s, const float* stats, const void* ds, const void* dh, void* dx,
+                               void* dy, void* dgate, void* d_post_w, void* d_post_b, void* d_pre_w, void* d_pre_b, float* scratch,
+                               void* stream);
 
 /* ---- input side ---------------------------------------------------------------------------------
  * NMS featuriser, src/datamodules/components/nms_dataset.py:23-61 + helper.py:16-59:
