@@ -29,6 +29,7 @@ EXPORTS = [
     "gcpnet_gcp2_weight_grads", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_stream_wait_stream", "gcpnet_wg_pack_multi",
     "gcpnet_grad_norm_partials", "gcpnet_grad_norm", "gcpnet_adamw_begin", "gcpnet_adamw_step",
     "gcpnet_block_norm_forward", "gcpnet_block_norm_backward", "gcpnet_block_norm_backward_scratch",
+    "gcpnet_linear_act_workspace", "gcpnet_linear_act_forward", "gcpnet_linear_act_backward",
 ]
 
 
@@ -99,6 +100,11 @@ class BlockNorm(C.Structure):
                 ("gate", C.c_void_p), ("x_ld", C.c_int64), ("y_ld", C.c_int64), ("gate_ld", C.c_int64), ("post_w", C.c_void_p),
                 ("post_b", C.c_void_p), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p), ("post", C.c_int), ("pre", C.c_int), ("act", C.c_int),
                 ("scale", C.c_float), ("slope", C.c_float), ("eps", C.c_float)]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("k", C.c_int), ("n", C.c_int), ("type", C.c_int), ("bias_type", C.c_int), ("act", C.c_int),
+                ("slope", C.c_float), ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("x_ld", C.c_int64), ("w_ld", C.c_int64)]
 
 
 class WgBwdPlan(C.Structure):
@@ -262,11 +268,15 @@ def load():
     lib.gcpnet_block_norm_backward.argtypes = [P(BlockNorm)] + [vp] * 13
     lib.gcpnet_block_norm_backward_scratch.argtypes = [i64, i32]
     lib.gcpnet_block_norm_backward_scratch.restype = i64
+    lib.gcpnet_linear_act_workspace.argtypes = [i64, i32, i32, i32, i32]
+    lib.gcpnet_linear_act_workspace.restype = i64
+    lib.gcpnet_linear_act_forward.argtypes = [P(LinearDesc), vp, i64, vp, vp, vp, vp]
+    lib.gcpnet_linear_act_backward.argtypes = [P(LinearDesc), vp, vp, i64] + [vp] * 6
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("gcpnet_gcp2_pack_floats", "gcpnet_layernorm_bwd_scratch_floats", "gcpnet_gcp2_forward_lds_bytes",
                         "gcpnet_wg_pack_floats", "gcpnet_tb_floats", "gcpnet_tb_sign_words", "gcpnet_gcp2_weight_grads_workspace", "gcpnet_grad_norm_partials",
-                        "gcpnet_block_norm_backward_scratch"):
+                        "gcpnet_block_norm_backward_scratch", "gcpnet_linear_act_workspace"):
             fn.restype = i32
     if lib.gcpnet_abi_version() != 4:
         raise GcpnetHipError("libgcpnet_hip.so ABI version mismatch")

@@ -1,5 +1,5 @@
-"""Operators of a residual block around its body, for fp32, bf16 and fp16 rows: the norms before and after it fused with its gate and
-residual scale (`residual_norm`).
+"""Operators of a residual block for fp32, bf16 and fp16 rows: a Linear with bias, activation and residual in its epilogue (`linear_act`), and
+the norms before and after a block fused with its gate and residual scale (`residual_norm`).
 
 As in `ops`: GPU tensors and libgcpnet_hip.so only, no fallback; the arithmetic between the loads and the stores is fp32."""
 from __future__ import annotations
@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import ACT, NORM, TYPE_BF16, TYPE_F16, TYPE_F32, BlockNorm, check
+from ._lib import ACT, NORM, TYPE_BF16, TYPE_F16, TYPE_F32, BlockNorm, LinearDesc, check
 from .ops import _stream
 
 Tensor = torch.Tensor
@@ -162,3 +162,77 @@ def residual_norm(x: Tensor, y: Optional[Tensor] = None, gate: Optional[Tensor] 
         first = w.dtype
     s, h = _ResidualNorm.apply((post, pre, gate_act, float(scale), float(slope), float(eps)), x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     return (x if y is None else s), h
+
+
+# ==============================================================================================================
+# Linear with bias, activation and residual
+# ==============================================================================================================
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cfg, x, weight, bias, residual):
+        act, slope = cfg
+        x2, w2, r2 = _rows(x), _rows(weight), None if residual is None else _rows(residual)
+        b2 = None if bias is None else bias.contiguous()
+        rows, k = x2.shape
+        n = w2.shape[0]
+        need = any(ctx.needs_input_grad[1:4])
+        q = LinearDesc()
+        q.rows, q.k, q.n, q.type, q.act, q.slope = rows, k, n, TYPES[x.dtype], ACT[act], slope
+        q.bias_type = q.type if b2 is None else TYPES[b2.dtype]
+        q.x, q.w, q.bias, q.x_ld, q.w_ld = x2.data_ptr(), w2.data_ptr(), _ptr(b2), x2.stride(0), w2.stride(0)
+        lib = _lib.load()
+        with _on(x):
+            y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+            z = torch.empty((rows, n), dtype=x.dtype, device=x.device) if need and act is not None else None
+            space = int(lib.gcpnet_linear_act_workspace(rows, k, n, q.type, 0))
+            ws = torch.empty(space, dtype=torch.float32, device=x.device) if space > 0 else None
+            check(lib.gcpnet_linear_act_forward(C.byref(q), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), _ptr(z), _ptr(ws), _stream()),
+                  "linear_act")
+        if need:
+            ctx.save_for_backward(x2, w2, z)
+            ctx.desc, ctx.shapes, ctx.bias_dtype = q, (x.shape, weight.shape), None if b2 is None else b2.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _, need_x, need_w, need_b, need_r = ctx.needs_input_grad
+        if not (need_x or need_w or need_b):
+            return None, None, None, None, dy if need_r else None
+        x2, w2, z = ctx.saved_tensors
+        q = ctx.desc
+        g2 = _rows(dy)
+        lib = _lib.load()
+        with _on(x2):
+            new = lambda shape, dtype=x2.dtype: torch.empty(shape, dtype=dtype, device=x2.device)  # noqa: E731
+            dx = new(ctx.shapes[0]) if need_x else None
+            dw = new(ctx.shapes[1]) if need_w else None
+            db = new((q.n,), ctx.bias_dtype) if need_b else None
+            dz = None if z is None else new((q.rows, q.n))
+            space = int(lib.gcpnet_linear_act_workspace(q.rows, q.k, q.n, q.type, 1))
+            ws = new((space,), torch.float32) if space > 0 else None
+            check(lib.gcpnet_linear_act_backward(C.byref(q), _ptr(z), g2.data_ptr(), g2.stride(0), _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+                                                 _stream()), "linear_act backward")
+        return None, dx, dw, db, dy if need_r else None
+
+
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Optional[str] = None, residual: Optional[Tensor] = None,
+               slope: float = 1e-2) -> Tensor:
+    """act(x @ weight^T + bias) + residual, rounded once: [..., k] x [n, k] -> [..., n] in one launch (two where k is split).
+
+    x, weight, residual: one type of fp32, bf16 and fp16; bias that type or fp32; act as in `get_nonlinearity` or None; any sizes from one row and
+    one column on.  Sums are fp32 (fp32 operands on the fp32 matrix instructions: no shorter terms).  Row strides are taken as they are, other
+    layouts are copied.  The backward keeps the pre-activation in x's type, and rounds its gradient to that type as an operand of the products for
+    x and weight; the bias gradient is summed unrounded.  All sums have a fixed order, so a run repeats bit for bit."""
+    _check_first(x, "x")
+    _check(weight, "weight", x)
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"linear_act: weight must be [n, {x.shape[-1]}] with at least one row and column, got {tuple(weight.shape)}")
+    if act not in ACT:
+        raise ValueError(f"linear_act: act is None or one of {sorted(k for k in ACT if k)}, got {act!r}")
+    n = weight.shape[0]
+    if bias is not None:
+        _check(bias, "bias", x, (n,), (x.dtype, torch.float32))
+    if residual is not None:
+        _check(residual, "residual", x, (*x.shape[:-1], n))
+    return _LinearAct.apply((act, float(slope)), x, weight, bias, residual)

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "elem_types.h"
+#include "linear_tiles.h"
 
 namespace {
 
@@ -382,6 +383,18 @@ bool whole_pieces(const gcp_block_norm_t* n, std::initializer_list<const void*> 
 
 }  // namespace
 
+int gcp_column_sums(const float* part, int blocks, int sets, int d, void* const* out, const int* type, hipStream_t stream) {
+    ColArgs c = {};
+    c.part = part; c.blocks = blocks; c.sets = sets; c.d = d;
+    for (int q = 0; q < sets; ++q) {
+        c.out[q] = out[q];
+        c.type[q] = type[q];
+    }
+    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)gcp_cdiv(d, 64), (unsigned)sets), dim3(1024), 0, stream, c);
+    GCP_HIP_CHECK_LAUNCH();
+    return 0;
+}
+
 extern "C" int gcpnet_block_norm_forward(const gcp_block_norm_t* n, void* s, void* h, float* stats, void* stream) {
     if (int rc = check_desc(n)) return rc;
     if (n->rows == 0) return 0;
@@ -417,12 +430,13 @@ extern "C" int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const void*
     const bool channel = n->gate && n->gate_ld == 0;
     void* const out[SETS] = {n->pre ? d_pre_w : nullptr, n->pre ? d_pre_b : nullptr, n->post ? d_post_w : nullptr, n->post ? d_post_b : nullptr,
                              channel ? dgate : nullptr};
-    ColArgs c = {};
+    void* sums[SETS];
+    int types[SETS];
     for (int q = 0; q < SETS; ++q) {
         a.slot[q] = out[q] ? a.sets : -1;
         if (!out[q]) continue;
-        c.out[a.sets] = out[q];
-        c.type[a.sets++] = q == 4 ? n->type : n->param_type;
+        sums[a.sets] = out[q];
+        types[a.sets++] = q == 4 ? n->type : n->param_type;
     }
     if (a.sets && n->rows > 0 && !scratch) return GCPNET_E_BADARG;
     int64_t blocks = 0;
@@ -448,10 +462,6 @@ extern "C" int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const void*
         });
         if (rc) return rc;
     }
-    if (a.sets) {  // (no rows: the sums are 0)
-        c.part = scratch; c.blocks = (int)blocks; c.sets = a.sets; c.d = n->d;
-        hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)gcp_cdiv(n->d, 64), (unsigned)a.sets), dim3(1024), 0, (hipStream_t)stream, c);
-        GCP_HIP_CHECK_LAUNCH();
-    }
+    if (a.sets) return gcp_column_sums(scratch, (int)blocks, a.sets, n->d, sums, types, (hipStream_t)stream);  // (no rows: the sums are 0)
     return 0;
 }

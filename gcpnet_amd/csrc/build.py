@@ -4,8 +4,8 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["gcp2_fwd.hip", "gcp2_chain_fwd.hip", "gcp2_bwd.hip", "gcp2_chain_bwd.hip", "tn_gemm.hip", "graph_ops.hip", "gcp_wg_fwd.hip", "gcp_wg_bwd.hip", "misc_ops.hip", "featurize.hip", "adamw.hip", "block_norm.hip"]
-HEADERS = ["common.h", "tile_io.h", "vec_mfma.h", "gcp_wg.h", "gcp_bf16x3.h", "gcp_f16x2.h", "elem_types.h", os.path.join("..", "..", "include", "gcpnet_hip.h")]
+SOURCES = ["gcp2_fwd.hip", "gcp2_chain_fwd.hip", "gcp2_bwd.hip", "gcp2_chain_bwd.hip", "tn_gemm.hip", "graph_ops.hip", "gcp_wg_fwd.hip", "gcp_wg_bwd.hip", "misc_ops.hip", "featurize.hip", "adamw.hip", "block_norm.hip", "linear_act.hip"]
+HEADERS = ["common.h", "tile_io.h", "vec_mfma.h", "gcp_wg.h", "gcp_bf16x3.h", "gcp_f16x2.h", "elem_types.h", "linear_tiles.h", os.path.join("..", "..", "include", "gcpnet_hip.h")]
 LIB = os.path.join(HERE, "libgcpnet_hip.so")
 # (-packed-fp32-ops: hipcc otherwise forms v_pk_{add,mul,fma}_f32 from ordinary float code, some forms of which have given wrong results
 # on these GPUs now and then; the host pass warns that it does not know the feature)
