@@ -23,9 +23,22 @@ def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(t: Tensor):
-    """The launches of an operator go to the device of its tensors, whatever the current one is."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    """The launches of an operator go to the device of its tensors, whatever the current one is.  (In a backward autograd has seen to it.)"""
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _backward(body):
+    """A backward that autograd may not differentiate again: with a graph asked for, the wrapper that makes such a use raise."""
+    once = once_differentiable(body)
+    return staticmethod(lambda ctx, *grads: once(ctx, *grads) if torch.is_grad_enabled() else body(ctx, *grads))
+
+
+def _wants_grad(tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -64,63 +77,74 @@ def _check_first(x, name: str) -> None:
 # ==============================================================================================================
 # norms before and after a block, with its gate and residual scale
 # ==============================================================================================================
+def _norm_forward(cfg, x, y, gate, weights, need):
+    """The launch: s, h, and what a backward keeps."""
+    post, pre, act, scale, slope, eps = cfg
+    x2 = _rows(x)
+    y2 = None if y is None else _rows(y)
+    channel = gate is not None and gate.dim() == 1
+    g2 = None if gate is None else gate.contiguous() if channel else _rows(gate)
+    rows, d = x2.shape
+    if g2 is not None and not channel and g2.stride(0) == 0 and rows > 1:
+        g2 = g2.contiguous()
+    ws = [None if w is None else w.contiguous() for w in weights]
+    n = BlockNorm()
+    n.rows, n.d, n.type = rows, d, TYPES[x.dtype]
+    n.param_type = next((TYPES[w.dtype] for w in ws if w is not None), n.type)
+    n.x, n.y, n.gate = x2.data_ptr(), _ptr(y2), _ptr(g2)
+    n.x_ld, n.y_ld, n.gate_ld = x2.stride(0), 0 if y2 is None else y2.stride(0), 0 if g2 is None or channel else d if rows == 1 else g2.stride(0)
+    n.post_w, n.post_b, n.pre_w, n.pre_b = map(_ptr, ws)
+    n.post, n.pre, n.act, n.scale, n.slope, n.eps = NORM[post], NORM[pre], ACT[act], scale, slope, eps
+    with _on(x):
+        s = x.new_empty(x.shape) if y is not None else None
+        h = x.new_empty(x.shape) if pre is not None else None
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if need and (post or pre) else None
+        check(_lib.load().gcpnet_block_norm_forward(C.byref(n), _ptr(s), _ptr(h), _ptr(stats), _stream()), "residual_norm")
+    return s, h, (n, channel, (y2, s if s is not None else x2, g2, stats, *ws))
+
+
+def _norm_backward(ctx, ds, dh):
+    y2, s, g2, stats, *ws = ctx.saved_tensors
+    shape, gate_shape = ctx.shapes
+    n = ctx.desc
+    if ds is None and dh is None:
+        return (None,) * 8
+    ds, dh = (None if g is None else g.contiguous() for g in (ds, dh))
+    _, need_x, need_y, need_gate, *need_w = ctx.needs_input_grad
+    b = BlockNorm.from_buffer_copy(n)  # (addresses anew: what was saved may have been elsewhere meanwhile)
+    b.x, b.x_ld = None, n.d if y2 is not None else s.stride(0)
+    b.y, b.gate = _ptr(y2), _ptr(g2)
+    b.post_w, b.post_b, b.pre_w, b.pre_b = map(_ptr, ws)
+    if y2 is not None:
+        b.y_ld = y2.stride(0)
+    if g2 is not None and not ctx.channel and n.rows > 1:
+        b.gate_ld = g2.stride(0)
+    lib = _lib.load()
+    new = lambda want, like: s.new_empty(like) if want else None  # noqa: E731
+    dx, dy, dgate = new(need_x, shape), new(need_y and y2 is not None, shape), new(need_gate and g2 is not None, gate_shape)
+    dws = [None] * 4
+    wanted = [i for i in range(4) if need_w[i] and ws[i] is not None]
+    if wanted:  # (one allocation: they are short)
+        for i, v in zip(wanted, ws[wanted[0]].new_empty((len(wanted), n.d)).unbind()):
+            dws[i] = v
+    scratch = None
+    if wanted or (dgate is not None and ctx.channel):
+        scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(n.rows, n.d))), dtype=torch.float32, device=s.device)
+    check(lib.gcpnet_block_norm_backward(C.byref(b), s.data_ptr(), _ptr(stats), _ptr(ds), _ptr(dh), _ptr(dx), _ptr(dy), _ptr(dgate),
+                                         *map(_ptr, dws), _ptr(scratch), _stream()), "residual_norm backward")
+    return (None, dx, dy, dgate, *dws)
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, cfg, x, y, gate, post_w, post_b, pre_w, pre_b):
-        post, pre, act, scale, slope, eps = cfg
-        x2 = _rows(x)
-        y2 = None if y is None else _rows(y)
-        channel = gate is not None and gate.dim() == 1
-        g2 = None if gate is None else gate.contiguous() if channel else _rows(gate)
-        rows, d = x2.shape
-        if g2 is not None and not channel and g2.stride(0) == 0 and rows > 1:
-            g2 = g2.contiguous()
-        ws = [None if w is None else w.contiguous() for w in (post_w, post_b, pre_w, pre_b)]
-        need = any(ctx.needs_input_grad)
-        n = BlockNorm()
-        n.rows, n.d, n.type = rows, d, TYPES[x.dtype]
-        n.param_type = next((TYPES[w.dtype] for w in ws if w is not None), n.type)
-        n.x, n.y, n.gate = x2.data_ptr(), _ptr(y2), _ptr(g2)
-        n.x_ld, n.y_ld, n.gate_ld = x2.stride(0), 0 if y2 is None else y2.stride(0), 0 if g2 is None or channel else d if rows == 1 else g2.stride(0)
-        n.post_w, n.post_b, n.pre_w, n.pre_b = (_ptr(w) for w in ws)
-        n.post, n.pre, n.act, n.scale, n.slope, n.eps = NORM[post], NORM[pre], ACT[act], scale, slope, eps
-        with _on(x):
-            s = x.new_empty(x.shape) if y is not None else None
-            h = x.new_empty(x.shape) if pre is not None else None
-            stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if need and (post or pre) else None
-            check(_lib.load().gcpnet_block_norm_forward(C.byref(n), _ptr(s), _ptr(h), _ptr(stats), _stream()), "residual_norm")
-        if need:
-            ctx.save_for_backward(y2, s if s is not None else x2, g2, stats, *ws)
-            ctx.desc, ctx.channel = n, channel
-            ctx.shapes = (x.shape, None if gate is None else gate.shape)
+    def forward(ctx, cfg, x, y, gate, *weights):
+        s, h, (ctx.desc, ctx.channel, keep) = _norm_forward(cfg, x, y, gate, weights, True)
+        ctx.save_for_backward(*keep)
+        ctx.shapes = (x.shape, None if gate is None else gate.shape)
         ctx.set_materialize_grads(False)
         return s, h
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, ds, dh):
-        y2, s, g2, stats, *ws = ctx.saved_tensors
-        shape, gate_shape = ctx.shapes
-        n = ctx.desc
-        none = (None,) * 8
-        if ds is None and dh is None:
-            return none
-        ds, dh = (None if g is None else g.contiguous() for g in (ds, dh))
-        _, need_x, need_y, need_gate, *need_w = ctx.needs_input_grad
-        s2 = s.view(n.rows, n.d) if s.is_contiguous() else s
-        b = BlockNorm.from_buffer_copy(n)
-        b.x, b.x_ld = None, s2.stride(0)
-        lib = _lib.load()
-        with _on(s):
-            new = lambda want, like: torch.empty(like, dtype=s.dtype, device=s.device) if want else None  # noqa: E731
-            dx, dy, dgate = new(need_x, shape), new(need_y and y2 is not None, shape), new(need_gate and g2 is not None, gate_shape)
-            dws = [torch.empty_like(w) if w is not None and want else None for w, want in zip(ws, need_w)]
-            scratch = None
-            if any(w is not None for w in dws) or (dgate is not None and ctx.channel):
-                scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(n.rows, n.d))), dtype=torch.float32, device=s.device)
-            check(lib.gcpnet_block_norm_backward(C.byref(b), s2.data_ptr(), _ptr(stats), _ptr(ds), _ptr(dh), _ptr(dx), _ptr(dy), _ptr(dgate),
-                                                 *(_ptr(w) for w in dws), _ptr(scratch), _stream()), "residual_norm backward")
-        return (None, dx, dy, dgate, *dws)
+    backward = _backward(_norm_backward)
 
 
 def residual_norm(x: Tensor, y: Optional[Tensor] = None, gate: Optional[Tensor] = None, *, scale: float = 1.0, gate_act: Optional[str] = None,
@@ -160,60 +184,68 @@ def residual_norm(x: Tensor, y: Optional[Tensor] = None, gate: Optional[Tensor] 
             raise ValueError(f"residual_norm: {name} without its norm")
         _check(w, name, x, (d,), (x.dtype, torch.float32) if first is None else (first,))
         first = w.dtype
-    s, h = _ResidualNorm.apply((post, pre, gate_act, float(scale), float(slope), float(eps)), x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+    cfg, weights = (post, pre, gate_act, float(scale), float(slope), float(eps)), (post_weight, post_bias, pre_weight, pre_bias)
+    if _wants_grad((x, y, gate, *weights)):
+        s, h = _ResidualNorm.apply(cfg, x, y, gate, *weights)
+    else:
+        s, h, _ = _norm_forward(cfg, x, y, gate, weights, False)
     return (x if y is None else s), h
 
 
 # ==============================================================================================================
 # Linear with bias, activation and residual
 # ==============================================================================================================
+def _linear_forward(cfg, x, weight, bias, residual, need):
+    """The launch: y, and what a backward keeps."""
+    act, slope = cfg
+    x2, w2, r2 = _rows(x), _rows(weight), None if residual is None else _rows(residual)
+    b2 = None if bias is None else bias.contiguous()
+    rows, k = x2.shape
+    n = w2.shape[0]
+    q = LinearDesc()
+    q.rows, q.k, q.n, q.type, q.act, q.slope = rows, k, n, TYPES[x.dtype], ACT[act], slope
+    q.bias_type = q.type if b2 is None else TYPES[b2.dtype]
+    q.x, q.w, q.bias, q.x_ld, q.w_ld = x2.data_ptr(), w2.data_ptr(), _ptr(b2), x2.stride(0), w2.stride(0)
+    lib = _lib.load()
+    with _on(x):
+        y = x.new_empty((*x.shape[:-1], n))
+        z = x.new_empty((rows, n)) if need and act is not None else None
+        space = lib.gcpnet_linear_act_workspace(rows, k, n, q.type, 0)
+        ws = torch.empty(space, dtype=torch.float32, device=x.device) if space > 0 else None
+        check(lib.gcpnet_linear_act_forward(C.byref(q), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), _ptr(z), _ptr(ws), _stream()),
+              "linear_act")
+    return y, q, (x2, w2, z)
+
+
+def _linear_backward(ctx, dy):
+    _, need_x, need_w, need_b, need_r = ctx.needs_input_grad
+    if not (need_x or need_w or need_b):
+        return None, None, None, None, dy if need_r else None
+    x2, w2, z = ctx.saved_tensors
+    q = LinearDesc.from_buffer_copy(ctx.desc)  # (addresses anew: what was saved may have been elsewhere meanwhile)
+    q.x, q.w, q.bias, q.x_ld, q.w_ld = x2.data_ptr(), w2.data_ptr(), None, x2.stride(0), w2.stride(0)
+    g2 = _rows(dy)
+    lib = _lib.load()
+    dx = x2.new_empty(ctx.shapes[0]) if need_x else None
+    dw = x2.new_empty(ctx.shapes[1]) if need_w else None
+    db = x2.new_empty(q.n, dtype=ctx.bias_dtype) if need_b else None
+    dz = None if z is None else x2.new_empty((q.rows, q.n))
+    space = lib.gcpnet_linear_act_workspace(q.rows, q.k, q.n, q.type, 1)
+    ws = x2.new_empty(space, dtype=torch.float32) if space > 0 else None
+    check(lib.gcpnet_linear_act_backward(C.byref(q), _ptr(z), g2.data_ptr(), g2.stride(0), _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+                                         _stream()), "linear_act backward")
+    return None, dx, dw, db, dy if need_r else None
+
+
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, x, weight, bias, residual):
-        act, slope = cfg
-        x2, w2, r2 = _rows(x), _rows(weight), None if residual is None else _rows(residual)
-        b2 = None if bias is None else bias.contiguous()
-        rows, k = x2.shape
-        n = w2.shape[0]
-        need = any(ctx.needs_input_grad[1:4])
-        q = LinearDesc()
-        q.rows, q.k, q.n, q.type, q.act, q.slope = rows, k, n, TYPES[x.dtype], ACT[act], slope
-        q.bias_type = q.type if b2 is None else TYPES[b2.dtype]
-        q.x, q.w, q.bias, q.x_ld, q.w_ld = x2.data_ptr(), w2.data_ptr(), _ptr(b2), x2.stride(0), w2.stride(0)
-        lib = _lib.load()
-        with _on(x):
-            y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-            z = torch.empty((rows, n), dtype=x.dtype, device=x.device) if need and act is not None else None
-            space = int(lib.gcpnet_linear_act_workspace(rows, k, n, q.type, 0))
-            ws = torch.empty(space, dtype=torch.float32, device=x.device) if space > 0 else None
-            check(lib.gcpnet_linear_act_forward(C.byref(q), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), _ptr(z), _ptr(ws), _stream()),
-                  "linear_act")
-        if need:
-            ctx.save_for_backward(x2, w2, z)
-            ctx.desc, ctx.shapes, ctx.bias_dtype = q, (x.shape, weight.shape), None if b2 is None else b2.dtype
+        y, ctx.desc, keep = _linear_forward(cfg, x, weight, bias, residual, any(ctx.needs_input_grad[1:4]))
+        ctx.save_for_backward(*keep)
+        ctx.shapes, ctx.bias_dtype = (x.shape, weight.shape), None if bias is None else bias.dtype
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        _, need_x, need_w, need_b, need_r = ctx.needs_input_grad
-        if not (need_x or need_w or need_b):
-            return None, None, None, None, dy if need_r else None
-        x2, w2, z = ctx.saved_tensors
-        q = ctx.desc
-        g2 = _rows(dy)
-        lib = _lib.load()
-        with _on(x2):
-            new = lambda shape, dtype=x2.dtype: torch.empty(shape, dtype=dtype, device=x2.device)  # noqa: E731
-            dx = new(ctx.shapes[0]) if need_x else None
-            dw = new(ctx.shapes[1]) if need_w else None
-            db = new((q.n,), ctx.bias_dtype) if need_b else None
-            dz = None if z is None else new((q.rows, q.n))
-            space = int(lib.gcpnet_linear_act_workspace(q.rows, q.k, q.n, q.type, 1))
-            ws = new((space,), torch.float32) if space > 0 else None
-            check(lib.gcpnet_linear_act_backward(C.byref(q), _ptr(z), g2.data_ptr(), g2.stride(0), _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
-                                                 _stream()), "linear_act backward")
-        return None, dx, dw, db, dy if need_r else None
+    backward = _backward(_linear_backward)
 
 
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Optional[str] = None, residual: Optional[Tensor] = None,
@@ -235,4 +267,6 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Op
         _check(bias, "bias", x, (n,), (x.dtype, torch.float32))
     if residual is not None:
         _check(residual, "residual", x, (*x.shape[:-1], n))
-    return _LinearAct.apply((act, float(slope)), x, weight, bias, residual)
+    if _wants_grad((x, weight, bias, residual)):
+        return _LinearAct.apply((act, float(slope)), x, weight, bias, residual)
+    return _linear_forward((act, float(slope)), x, weight, bias, residual, False)[0]

@@ -150,7 +150,15 @@ class _Part:
         self.type = _lib.TYPE_F32 if dtype == torch.float32 else _lib.TYPE_BF16
         self.params = [p for p, _, _, _ in items]
         self.arr = (AdamWTensor * len(items))()
-        self.known, self.copies = [], []
+        self.copies = []
+        # what the next step compares with (strong references: an id stays its object's); a permuted parameter never matches, its table is
+        # built anew every step
+        self.states = [st for _, _, st, _ in items]
+        self.held = [v for st in self.states for v in st.values()]
+        self.ids = [id(v) for v in self.held]
+        self.live, self.order = [id(p) for p in self.params], [ordinal for _, _, _, ordinal in items]
+        self.addresses = [p.data_ptr() if p.is_contiguous() else None for p in self.params]
+        self.sizes = [p.numel() for p in self.params]
         for t, (p, g, st, ordinal) in zip(self.arr, items):
             if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
                 g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
@@ -161,8 +169,7 @@ class _Part:
                 t.exp_avg_scale, t.exp_avg_sq_scale = st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()
             if dtype == torch.bfloat16:
                 t.master = st["master"].data_ptr()
-            # (a permuted parameter never matches: its table is built anew every step)
-            self.known.append((p, p.data_ptr() if p.is_contiguous() else None, p.numel(), tuple(map(id, st.values())), tuple(st.values())))
+        self.grads = [t.grad for t in self.arr]
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -189,7 +196,7 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed))
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None
-        self._parts = {}
+        self._parts, self._state_ids = {}, []
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -222,7 +229,7 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
-        self._parts = {}
+        self._parts, self._state_ids = {}, []
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
@@ -231,7 +238,7 @@ class FusedAdamW(torch.optim.Optimizer):
         """torch's loader converts every state tensor to its parameter's type: here the moments, scales and master copies keep theirs.
         Moments of another kind (fp32 for a group with 8 bits, or the reverse) are refused."""
         super().load_state_dict(state_dict)
-        self._parts = {}
+        self._parts, self._state_ids = {}, []
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for g in self.param_groups:  # (state of groups written by torch.optim.AdamW has no such keys)
             g.setdefault("state_bits", self.defaults["state_bits"])
@@ -313,16 +320,21 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         lib = _lib.load()
-        devices, touched, ordinal = {}, [], 0  # device index -> [(group, _Part)]
+        if list(map(id, self.state.values())) != self._state_ids:  # (a state was put in, taken out or exchanged)
+            self._parts = {}
+        devices, touched, ordinal, built = {}, [], 0, False  # device index -> [(group, _Part)]
         for gi, group in enumerate(self.param_groups):
             self._check_options(group)
             parts = self._parts.get(gi)
             if parts is None or parts[0] != (ordinal, group["state_bits"]) or not self._refresh(parts[1], group["params"]):
                 parts = self._parts[gi] = ((ordinal, group["state_bits"]), self._build(group, ordinal))
+                built = True
             ordinal += len(group["params"])
             for part in parts[1]:
                 devices.setdefault(part.device, []).append((group, part))
-                touched += part.params
+                touched.extend(part.params)
+        if built:
+            self._state_ids = list(map(id, self.state.values()))
         if len(devices) > 1 and self.max_grad_norm is not None:
             raise _lib.GcpnetHipError("FusedAdamW: max_grad_norm with parameters on several devices is not supported")
         for dev, parts in devices.items():
@@ -331,9 +343,10 @@ class FusedAdamW(torch.optim.Optimizer):
         if touched:
             torch.autograd.graph.increment_version(touched)  # (written through raw pointers: autograd's and the packs' caches must notice)
             ops.invalidate_packs()
-        for _, parts in self._parts.values():
-            for part in parts:
-                part.copies.clear()
+        if built:
+            for _, parts in self._parts.values():
+                for part in parts:
+                    part.copies.clear()
         return loss
 
     def _build(self, group, ordinal):
@@ -364,19 +377,27 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _refresh(self, parts, params) -> bool:
         """Whether the same parameters take part with the same state as when `parts` were built; puts this step's gradients in."""
-        live = [id(p) for p in params if p.grad is not None]
-        if sorted(live) != sorted(id(p) for part in parts for p in part.params):
+        grads = [p.grad for p in params]
+        if [id(p) for p, g in zip(params, grads) if g is not None] != self._live(parts):
             return False
-        state = self.state
         for part in parts:
-            arr, dtype = part.arr, part.dtype
-            for k, (p, address, n, ids, _) in enumerate(part.known):
-                g = p.grad
-                if (g is None or not g.is_contiguous() or g.dtype is not dtype or g.numel() != n or p.data_ptr() != address
-                        or tuple(map(id, state[p].values())) != ids):
-                    return False
-                arr[k].grad = g.data_ptr()
+            ps, dtype = part.params, part.dtype
+            grads = [p.grad for p in ps]
+            if ([p.data_ptr() for p in ps] != part.addresses or [g.numel() for g in grads] != part.sizes or any([g.dtype is not dtype for g in grads])
+                    or not all([g.is_contiguous() for g in grads]) or [id(v) for st in part.states for v in st.values()] != part.ids):
+                return False
+            pointers = [g.data_ptr() for g in grads]
+            if pointers != part.grads:
+                for t, g in zip(part.arr, pointers):
+                    t.grad = g
+                part.grads = pointers
         return True
+
+    @staticmethod
+    def _live(parts):
+        if len(parts) == 1:
+            return parts[0].live
+        return [i for _, i in sorted((k, i) for part in parts for k, i in zip(part.order, part.live))]
 
     def _step_device(self, lib, dev, parts):
         stream, where = ops._stream(), torch.device("cuda", dev)

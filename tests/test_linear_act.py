@@ -224,6 +224,22 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.gpu
+def test_saved_tensors_that_went_to_the_host_and_second_derivatives():
+    x, w, b, r, dy = make(50, 64, 72, torch.bfloat16)
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    want = torch.autograd.grad(G.linear_act(x, w, b, act="silu", residual=r), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = G.linear_act(x, w, b, act="silu", residual=r)
+    torch.empty(1 << 20, device="cuda").fill_(math.nan)
+    for p, q in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(p, q)
+    got = torch.autograd.grad(G.linear_act(x, w, b, act="silu", residual=r), leaves, dy, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with pytest.raises(RuntimeError):
+        got[0].sum().backward()
+
+
+@pytest.mark.gpu
 def test_repeats_captured_and_on_another_stream():
     """A split product (few tiles, long k) and a large one, bit for bit from run to run, on another stream, and in replays of a graph."""
     for rows, k, n in ((40, 4096, 72), (700, 256, 520)):

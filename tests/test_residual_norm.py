@@ -289,6 +289,22 @@ def test_no_rows_one_row_and_repeats():
 
 
 @pytest.mark.gpu
+def test_saved_tensors_that_went_to_the_host_and_second_derivatives():
+    ten, ds, dh = make(20, 64, torch.float32, "element", "rms", "layer", 2)
+    names = list(ten)
+    call = lambda: G.residual_norm(**ten, gate_act="silu", post="rms", pre="layer")  # noqa: E731
+    want = torch.autograd.grad(call(), [ten[k] for k in names], (ds, dh))
+    with torch.autograd.graph.save_on_cpu():
+        out = call()
+    for p, q in zip(torch.autograd.grad(out, [ten[k] for k in names], (ds, dh)), want):
+        assert torch.equal(p, q)
+    got = torch.autograd.grad(call(), [ten[k] for k in names], (ds, dh), create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with pytest.raises(RuntimeError):
+        got[0].sum().backward()
+
+
+@pytest.mark.gpu
 def test_infinities_stay_in_their_rows():
     x, y = torch.randn(6, 32, device="cuda"), torch.randn(6, 32, device="cuda")
     y[2, 3], x[4, 0] = math.inf, math.nan
