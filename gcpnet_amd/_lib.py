@@ -268,10 +268,10 @@ def load():
     lib.gcpnet_block_norm_backward.argtypes = [P(BlockNorm)] + [vp] * 13
     lib.gcpnet_block_norm_backward_scratch.argtypes = [i64, i32]
     lib.gcpnet_block_norm_backward_scratch.restype = i64
-    lib.gcpnet_linear_act_workspace.argtypes = [i64, i32, i32, i32, i32]
+    lib.gcpnet_linear_act_workspace.argtypes = [P(LinearDesc), i32]
     lib.gcpnet_linear_act_workspace.restype = i64
     lib.gcpnet_linear_act_forward.argtypes = [P(LinearDesc), vp, i64, vp, vp, vp, vp]
-    lib.gcpnet_linear_act_backward.argtypes = [P(LinearDesc), vp, vp, i64] + [vp] * 6
+    lib.gcpnet_linear_act_backward.argtypes = [P(LinearDesc), vp, vp, i64] + [vp] * 5
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("gcpnet_gcp2_pack_floats", "gcpnet_layernorm_bwd_scratch_floats", "gcpnet_gcp2_forward_lds_bytes",

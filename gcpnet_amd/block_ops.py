@@ -210,7 +210,7 @@ def _linear_forward(cfg, x, weight, bias, residual, need):
     with _on(x):
         y = x.new_empty((*x.shape[:-1], n))
         z = x.new_empty((rows, n)) if need and act is not None else None
-        space = lib.gcpnet_linear_act_workspace(rows, k, n, q.type, 0)
+        space = lib.gcpnet_linear_act_workspace(C.byref(q), 0)
         ws = torch.empty(space, dtype=torch.float32, device=x.device) if space > 0 else None
         check(lib.gcpnet_linear_act_forward(C.byref(q), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), _ptr(z), _ptr(ws), _stream()),
               "linear_act")
@@ -229,10 +229,9 @@ def _linear_backward(ctx, dy):
     dx = x2.new_empty(ctx.shapes[0]) if need_x else None
     dw = x2.new_empty(ctx.shapes[1]) if need_w else None
     db = x2.new_empty(q.n, dtype=ctx.bias_dtype) if need_b else None
-    dz = None if z is None else x2.new_empty((q.rows, q.n))
-    space = lib.gcpnet_linear_act_workspace(q.rows, q.k, q.n, q.type, 1)
+    space = lib.gcpnet_linear_act_workspace(C.byref(q), 1)
     ws = x2.new_empty(space, dtype=torch.float32) if space > 0 else None
-    check(lib.gcpnet_linear_act_backward(C.byref(q), _ptr(z), g2.data_ptr(), g2.stride(0), _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+    check(lib.gcpnet_linear_act_backward(C.byref(q), _ptr(z), g2.data_ptr(), g2.stride(0), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
                                          _stream()), "linear_act backward")
     return None, dx, dw, db, dy if need_r else None
 

@@ -6,15 +6,18 @@
 // dW), in one kernel template:
 //   * a workgroup owns a BM x BN tile of C, a wave a part of it in 16 x 16 MFMA tiles (16-bit: v_mfma_f32_16x16x32, fp32:
 //     v_mfma_f32_16x16x4_f32; sums in fp32);
-//   * tiles of 128 bytes of k travel from memory into one of two LDS buffers by direct loads (no registers), one tile ahead of the
-//     products; the 16-byte pieces of an LDS row are permuted (by the row) so that fragment reads spread over the banks;
+//   * tiles of 128 bytes of k travel from memory into a ring of LDS buffers by direct loads (no registers); the 16-byte pieces of an LDS
+//     row are permuted (by the row) so that fragment reads spread over the banks;
+//   * a tile is two steps of the 16-bit matrix instructions; while one step's fragments are multiplied the next step's are read, B's into
+//     a second set of registers, A's into the registers of the row of products just issued; the waves meet once a tile;
 //   * an operand with k across memory keeps its layout in LDS, [k][m]; 16-bit fragments come out of it through the transposing LDS
 //     read, fp32 ones element by element;
-//   * operands whose rows do not start at multiples of 16 bytes, and the tile in which k ends, go through registers element by element
-//     into the same places, zeros where there is no data;
+//   * operands whose rows are not whole 16-byte pieces are first copied into the workspace, rows filled up with zeros (one launch for all of
+//     them); where k ends inside a tile, the places behind it are set to zero;
 //   * few tiles of C: k is split over workgroups, which leave fp32 partial sums for a second launch that adds them in a fixed order and
 //     applies the epilogue (no atomics: results repeat bit for bit).
-// The epilogue adds the bias, applies the activation, adds the residual and rounds once; in training it also stores z.
+// The epilogue adds the bias, applies the activation, adds the residual and rounds once; in training it also stores z.  The accumulators go
+// through LDS first, so that a lane holds 16 bytes of a row and a wave reads and writes whole rows of its part of the tile.
 #include <type_traits>
 
 #include "elem_types.h"
@@ -33,7 +36,7 @@ constexpr int KROW = 128;  // bytes of k in a tile
 struct Epilogue {
     const void *bias, *residual;
     int64_t r_ld;
-    int act, bias_f32, whole;  // whole: four columns at a time (all rows of y, z, residual allow it)
+    int act, bias_f32, whole;  // whole: 16 bytes at a time (all rows of y, z, residual allow it)
     float slope;
     void *y, *z;  // contiguous [m, n]
 };
@@ -42,61 +45,77 @@ struct Gemm {
     int64_t m, n, k;
     const void *a, *b;
     int64_t a_ld, b_ld;
-    int a_fast, b_fast;  // 16-byte pieces
+    int64_t a_rows, b_rows;  // rows of A and B that are there to be read: m and n, or more where k is across and rows are filled up
     int tiles_m, tiles_n, splits;
     int64_t k_per;       // k per split, a multiple of the tile's
     float* part;         // [splits, m, n] or NULL
     Epilogue e;
 };
 
-template <class E>
-__device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t m, int64_t n, int64_t N, f32x4 v) {
-    typedef typename E::type T;
-    const int64_t at = m * N + n;
-    float out[4];
+// act of V values; the choice is uniform and made once for all of them.  (The reciprocal is good to a unit in the last place of fp32.)
+template <int V>
+__device__ __forceinline__ void act_all(int act, float slope, float (&v)[V]) {
+    if (act == GCP_ACT_NONE) return;
+    if (act == GCP_ACT_RELU || act == GCP_ACT_LEAKYRELU) {
+        const float low = act == GCP_ACT_RELU ? 0.f : slope;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = v[j];
-    const int cols = N - n < 4 ? (int)(N - n) : 4;
-    if (e.bias) {
+        for (int j = 0; j < V; ++j) v[j] = v[j] > 0.f ? v[j] : (low == 0.f ? 0.f : low * v[j]);
+    } else if (act == GCP_ACT_SELU) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cols) out[j] += (E::code != GCP_TYPE_F32 && e.bias_f32) ? ((const float*)e.bias)[n + j] : (float)((const T*)e.bias)[n + j];
-    }
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    if (e.z) {
-        if (e.whole) {
-            T4 q;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = (T)out[j];
-            *(T4*)((T*)e.z + at) = q;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < cols) ((T*)e.z)[at + j] = (T)out[j];
-        }
-    }
-    if (e.act != GCP_ACT_NONE) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out[j] = gcp_act(e.act, out[j], e.slope);
-    }
-    if (e.whole) {
-        if (e.residual) {
-            const T4 r = *(const T4*)((const T*)e.residual + m * e.r_ld + n);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[j] += (float)r[j];
-        }
-        T4 q;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = (T)out[j];
-        *(T4*)((T*)e.y + at) = q;
+        for (int j = 0; j < V; ++j) v[j] = gcp_act(GCP_ACT_SELU, v[j], slope);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cols) {
-                if (e.residual) out[j] += (float)((const T*)e.residual)[m * e.r_ld + n + j];
-                ((T*)e.y)[at + j] = (T)out[j];
+        for (int j = 0; j < V; ++j) {
+            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-v[j]));
+            v[j] = act == GCP_ACT_SILU ? v[j] * s : s;
+        }
+    }
+}
+
+// V columns of one row from n on: bias, z, activation, residual (`r`, loaded before, where the rows are whole), y
+template <class E, int V>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, int64_t N, const float (&bias)[V], const Raw<E, V>& r, float (&v)[V]) {
+    typedef typename E::type T;
+    const int64_t at = m * N + n;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += bias[j];
+    if (e.whole) {
+        if (e.z) elem_store<E, V>(e.z, at, v);
+        act_all<V>(e.act, e.slope, v);
+        if (e.residual)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] += (float)r.x[j];
+        elem_store<E, V>(e.y, at, v);
+    } else {
+        if (e.z)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (n + j < N) ((T*)e.z)[at + j] = (T)v[j];
+        act_all<V>(e.act, e.slope, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (n + j < N) {
+                if (e.residual) v[j] += (float)((const T*)e.residual)[m * e.r_ld + n + j];
+                ((T*)e.y)[at + j] = (T)v[j];
             }
     }
+}
+
+template <class E, int V>
+__device__ __forceinline__ void bias_load(const Epilogue& e, int64_t n, int64_t N, float (&bias)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = 0.f;
+        if (e.bias && n + j < N)
+            bias[j] = (E::code != GCP_TYPE_F32 && e.bias_f32) ? ((const float*)e.bias)[n + j] : (float)((const typename E::type*)e.bias)[n + j];
+    }
+}
+
+// 16 bytes per lane from memory (uniform base + offset) to LDS (lane l to base + 16 l), counted by vmcnt.  In asm, because the compiler would
+// otherwise wait for it before every later LDS read, which is of the other buffer; m0 it sets itself before each use.  (A write of m0 needs one wait state before its use.)
+__device__ __forceinline__ void to_lds(const char* from, unsigned offset, const char* lds) {
+    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(base), "v"(offset), "s"(from) : "memory");
 }
 
 // One operand's tile in LDS: R rows of C's side (m or n), KROW bytes of k.
@@ -122,42 +141,37 @@ struct Tile {
         piece = place(row, id % ROWP);  // (an involution)
     }
 
-    // address of the piece in memory at k = 0 of the tile; rows past the end are clamped (their products are never stored)
-    __device__ static __forceinline__ const char* address(const void* base, int64_t ld, int64_t first, int64_t rows, int64_t k0, int id) {
+    // the tile's first element in memory (uniform), and the piece's bytes from there (the host has seen that they fit 32 bits); rows past the
+    // end are clamped (their products are never stored)
+    __device__ static __forceinline__ const char* origin(const void* base, int64_t ld, int64_t first, int64_t k0) {
+        return (const char*)base + (ACROSS ? k0 * ld + first : first * ld + k0) * S;
+    }
+    __device__ static __forceinline__ unsigned offset(int64_t ld, int64_t first, int64_t rows, int id) {
         int row, piece;
         where(id, row, piece);
-        if constexpr (!ACROSS) {
-            int64_t i = first + row;
-            i = i < rows ? i : rows - 1;
-            return (const char*)base + (i * ld + k0 + piece * PE) * S;
-        } else {
-            int64_t i = first + piece * PE;
-            i = i < rows ? i : rows - PE;
-            return (const char*)base + ((k0 + row) * ld + i) * S;
-        }
+        const int64_t left = rows - first;  // (at least one row or piece)
+        if constexpr (!ACROSS) return (unsigned)(((row < left ? row : left - 1) * ld + piece * PE) * S);
+        else return (unsigned)((row * ld + (piece * PE < left ? piece * PE : left - PE)) * S);
     }
 
-    // element by element through registers: any address, any end
-    __device__ static void slow(char* lds, const void* base, int64_t ld, int64_t first, int64_t rows, int64_t k0, int64_t k_end) {
-#pragma unroll 1
-        for (int t = 0; t < TURNS; ++t) {
-            const int id = t * THREADS + (int)threadIdx.x;
-            int row, piece;
-            where(id, row, piece);
-            T x[PE];
+    // the tile from memory; `left`: k from its start on
+    template <bool WHOLE>
+    __device__ static __forceinline__ void stage(char* lds, const char* from, const unsigned (&offsets)[TURNS], int64_t left) {
+        const int wave = threadIdx.x >> 6;
 #pragma unroll
-            for (int j = 0; j < PE; ++j) {
-                const int64_t i = ACROSS ? first + piece * PE + j : first + row, k = ACROSS ? k0 + row : k0 + piece * PE + j;
-                x[j] = i < rows && k < k_end ? ((const T*)base)[ACROSS ? k * ld + i : i * ld + k] : (T)0.f;
+        for (int t = 0; t < TURNS; ++t) {
+            if constexpr (WHOLE) {
+                to_lds(from, offsets[t], lds + (t * THREADS + wave * 64) * 16);
+            } else {
+                int row, piece;
+                where(t * THREADS + (int)threadIdx.x, row, piece);
+                if ((ACROSS ? row : piece * PE) < left) to_lds(from, offsets[t], lds + (t * THREADS + wave * 64) * 16);
+                else *(u32x4*)(lds + (t * THREADS + (int)threadIdx.x) * 16) = u32x4{0, 0, 0, 0};
             }
-            u32x4 q;
-            __builtin_memcpy(&q, x, 16);
-            *(u32x4*)(lds + id * 16) = q;
         }
     }
 
-    // fragment of MFMA rows i0 .. i0 + 15 and k step `kk` (64 bytes of k each): 16 bytes per lane, lane l = 16 q + i: row i0 + i,
-    // k = (4 kk + q) pieces
+    // fragment of MFMA rows i0 .. i0 + 15 for step kk: 16 bytes per lane, lane l = 16 q + i: row i0 + i, piece 4 kk + q of its k
     __device__ static __forceinline__ u32x4 fragment(const char* lds, int i0, int kk, int lane) {
         const int i = lane & 15, q = lane >> 4;
         if constexpr (!ACROSS) {
@@ -197,19 +211,18 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     }
 }
 
-// 16 bytes per lane from memory to LDS (lane l to base + 16 l, the base uniform), counted by vmcnt.  In asm, because the compiler would
-// otherwise wait for it before every later LDS read, which is of the other buffer; m0 it sets itself before each use.  (A write of m0 needs one wait state before its use.)
-__device__ __forceinline__ void to_lds(const char* from, const char* lds) {
-    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(from) : "memory");
+template <int N>
+__device__ __forceinline__ void wait_loads_and_meet() {  // this wave's direct loads but the last N, and its LDS traffic; then all waves
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <class E, bool AC, bool BC, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(Gemm g) {
+template <class E, bool AC, bool BC, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
     constexpr int THREADS = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
     typedef Tile<E, AC, BM, THREADS> TA;
     typedef Tile<E, BC, BN, THREADS> TB;
-    __shared__ __attribute__((aligned(16))) char lds[2][TA::BYTES + TB::BYTES];
+    constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::TURNS + TB::TURNS;
+    __shared__ __attribute__((aligned(16))) char lds[RING * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
 
     const int total = g.tiles_m * g.tiles_n;
@@ -218,31 +231,25 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(Gemm g) {
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
     const int64_t k0 = (int64_t)blockIdx.y * g.k_per, k1 = k0 + g.k_per < g.k ? k0 + g.k_per : g.k;
     const int steps = k1 > k0 ? (int)((k1 - k0 + TA::KE - 1) / TA::KE) : 0;
+    const int whole = steps > 0 ? (int)((k1 - k0) / TA::KE) : 0;  // tiles that do not reach past the end of k
 
-    const char *pa[TA::TURNS], *pb[TB::TURNS];
-    if (g.a_fast)
+    const char *pa = TA::origin(g.a, g.a_ld, m0, k0), *pb = TB::origin(g.b, g.b_ld, n0, k0);
+    unsigned oa[TA::TURNS], ob[TB::TURNS];
 #pragma unroll
-        for (int t = 0; t < TA::TURNS; ++t) pa[t] = TA::address(g.a, g.a_ld, m0, g.m, k0, t * THREADS + tid);
-    if (g.b_fast)
+    for (int t = 0; t < TA::TURNS; ++t) oa[t] = TA::offset(g.a_ld, m0, g.a_rows, t * THREADS + tid);
 #pragma unroll
-        for (int t = 0; t < TB::TURNS; ++t) pb[t] = TB::address(g.b, g.b_ld, n0, g.n, k0, t * THREADS + tid);
+    for (int t = 0; t < TB::TURNS; ++t) ob[t] = TB::offset(g.b_ld, n0, g.b_rows, t * THREADS + tid);
     const int64_t da = (AC ? g.a_ld * TA::KE : TA::KE) * TA::S, db = (BC ? g.b_ld * TB::KE : TB::KE) * TB::S;
 
     auto stage = [&](int step, char* buf) {
-        const int64_t k = k0 + (int64_t)step * TA::KE;
-        const bool full = k + TA::KE <= k1;
-        if (g.a_fast && full) {
-#pragma unroll
-            for (int t = 0; t < TA::TURNS; ++t) { to_lds(pa[t], buf + (t * THREADS + wave * 64) * 16); pa[t] += da; }
+        const char *fa = pa + step * da, *fb = pb + step * db;
+        if (step < whole) {
+            TA::template stage<true>(buf, fa, oa, 0);
+            TB::template stage<true>(buf + TA::BYTES, fb, ob, 0);
         } else {
-            TA::slow(buf, g.a, g.a_ld, m0, g.m, k, k1);
-        }
-        buf += TA::BYTES;
-        if (g.b_fast && full) {
-#pragma unroll
-            for (int t = 0; t < TB::TURNS; ++t) { to_lds(pb[t], buf + (t * THREADS + wave * 64) * 16); pb[t] += db; }
-        } else {
-            TB::slow(buf, g.b, g.b_ld, n0, g.n, k, k1);
+            const int64_t left = k1 - k0 - (int64_t)step * TA::KE;
+            TA::template stage<false>(buf, fa, oa, left);
+            TB::template stage<false>(buf + TA::BYTES, fb, ob, left);
         }
     };
 
@@ -251,46 +258,104 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(Gemm g) {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (steps > 0) stage(0, lds[0]);
-    for (int s = 0; s < steps; ++s) {
-        // this tile has landed, everywhere; nobody reads the other buffer any more
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (s + 1 < steps) stage(s + 1, lds[(s + 1) & 1]);
-        const char *la = lds[s & 1], *lb = la + TA::BYTES;
+    u32x4 fa[TM], fb[2][TN];
+    auto read_b = [&](const char* buf, auto kk) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            u32x4 fa[TM], fb[TN];
+        for (int j = 0; j < TN; ++j) fb[kk][j] = TB::fragment(buf + TA::BYTES, (wn * TN + j) * 16, kk, lane);
+    };
+    auto read_a = [&](const char* buf, int kk, int i) { fa[i] = TA::fragment(buf, (wm * TM + i) * 16, kk, lane); };
+    auto multiply = [&](auto kk, const char* buf, int then) {  // the products of step kk; fragments of A for step `then` of buf
 #pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j] = TB::fragment(lb, (wn * TN + j) * 16, kk, lane);
+        for (int i = 0; i < TM; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) fa[i] = TA::fragment(la, (wm * TM + i) * 16, kk, lane);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mfma<E>(fb[j], fa[i], acc[i][j]);  // (transposed: a lane gets four n of one m)
+            for (int j = 0; j < TN; ++j) acc[i][j] = mfma<E>(fb[kk][j], fa[i], acc[i][j]);  // (transposed: a lane gets four n of one m)
+            __builtin_amdgcn_sched_barrier(0);  // (not before: the registers are the products')
+            read_a(buf, then, i);
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    std::integral_constant<int, 0> first;
+    std::integral_constant<int, 1> second;
+#pragma unroll 1
+    for (int t = 0; t < RING && t < steps; ++t) stage(t, lds + t * STAGE);
+    if (RING <= whole) wait_loads_and_meet<(RING - 1) * LOADS>();
+    else wait_loads_and_meet<0>();
+    char* buf = lds;
+    read_b(buf, first);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) read_a(buf, 0, i);
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        char* next = buf + STAGE == lds + RING * STAGE ? lds : buf + STAGE;
+        read_b(buf, second);
+        multiply(first, buf, 1);
+        // everybody has all of this tile's fragments, and the next tile is there: those after it may still be under way
+        if (s + RING <= whole) wait_loads_and_meet<(RING - 2) * LOADS>();
+        else wait_loads_and_meet<0>();
+        read_b(next, first);  // (behind the last tile: what is there is read, and not used)
+        if (s + RING < steps) stage(s + RING, buf);
+        multiply(second, next, 0);
+        buf = next;
     }
+    __syncthreads();  // (the epilogue writes over the ring)
 
-    const int q = lane >> 4;
+    // A wave's part of C goes through its own LDS, PH rows at a time: [PH][COLS] fp32 in pieces of 16 bytes, piece p of row r at p ^ (r & mask)
+    constexpr int COLS = TN * 16, P = COLS / 4, OWN = RING * STAGE / (WM * WN), ROWS = TM * 16;
+    constexpr int PH = ROWS * COLS * 4 <= OWN ? ROWS : OWN / (COLS * 4) / 16 * 16;
+    constexpr int V = E::vec, LPR = COLS / V, RPP = 64 / LPR;  // lanes per row, rows per pass
+    constexpr int AT_ONCE = PH / RPP < 4 ? PH / RPP : 4;
+    static_assert(PH >= 16 && ROWS % PH == 0 && PH % (RPP * AT_ONCE) == 0, "whole phases");
+    f32x4* own = (f32x4*)(lds + wave * OWN);
+    const int64_t n = n0 + wn * COLS + (lane % LPR) * V;
+    float bias[V];
+    bias_load<E, V>(g.e, n, g.n, bias);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int64_t m = m0 + (wm * TM + i) * 16 + (lane & 15);
-        if (m >= g.m) continue;
+    for (int ph = 0; ph < ROWS / PH; ++ph) {
+        gcp_wave_lds_sync();  // (lanes exchange: what the phase before read has been read)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int64_t n = n0 + (wn * TN + j) * 16 + 4 * q;
-            if (n >= g.n) continue;
-            if (g.part) {
-                float* p = g.part + ((int64_t)blockIdx.y * g.m + m) * g.n + n;
-                if (g.n % 4 == 0) *(f32x4*)p = acc[i][j];
-                else
+        for (int i = 0; i < PH / 16; ++i)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (n + c < g.n) p[c] = acc[i][j][c];
-            } else {
-                epilogue4<E>(g.e, m, n, g.n, acc[i][j]);
+            for (int j = 0; j < TN; ++j) {
+                const int r = i * 16 + (lane & 15);
+                own[r * P + ((4 * j + (lane >> 4)) ^ (r & (P - 1)))] = acc[ph * (PH / 16) + i][j];
+            }
+        gcp_wave_lds_sync();
+#pragma unroll 1
+        for (int r0 = 0; r0 < PH; r0 += RPP * AT_ONCE) {
+            // (the residual of several passes is requested before the first is finished)
+            Raw<E, V> res[AT_ONCE];
+            if (g.e.residual && g.e.whole && !g.part)
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    const int64_t m = m0 + wm * ROWS + ph * PH + r0 + u * RPP + lane / LPR;
+                    if (m < g.m && n < g.n) res[u] = elem_load<E, V>(g.e.residual, m * g.e.r_ld + n);
+                }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int r = r0 + u * RPP + lane / LPR;
+                const int64_t m = m0 + wm * ROWS + ph * PH + r;
+                float v[V];
+#pragma unroll
+                for (int h = 0; h < V / 4; ++h) {
+                    const f32x4 x = own[r * P + (((lane % LPR) * (V / 4) + h) ^ (r & (P - 1)))];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
+                }
+                if (m >= g.m || n >= g.n) continue;
+                if (g.part) {
+                    float* p = g.part + ((int64_t)blockIdx.y * g.m + m) * g.n + n;
+                    if (g.n % V == 0) {
+#pragma unroll
+                        for (int h = 0; h < V / 4; ++h) *(f32x4*)(p + 4 * h) = f32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            if (n + j < g.n) p[j] = v[j];
+                    }
+                } else {
+                    finish<E, V>(g.e, m, n, g.n, bias, res[u], v);
+                }
             }
         }
     }
@@ -299,21 +364,33 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(Gemm g) {
 // The partial sums of a split product, added in order, and the epilogue.
 template <class E>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t m, int64_t n, Epilogue e) {
-    const int64_t quads = (n + 3) / 4, all = m * quads;
+    constexpr int V = E::vec;
+    const int64_t vecs = (n + V - 1) / V, all = m * vecs, step = m * n;
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += (int64_t)gridDim.x * 256) {
-        const int64_t row = id / quads, col = (id - row * quads) * 4;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        const int64_t row = id / vecs, col = (id - row * vecs) * V;
+        float v[V], bias[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = 0.f;
         const float* p = part + row * n + col;
-        if (n % 4 == 0) {
+        bias_load<E, V>(e, col, n, bias);
+        if (n % V == 0) {
 #pragma unroll 4
-            for (int s = 0; s < splits; ++s) v += *(const f32x4*)(p + (int64_t)s * m * n);
+            for (int s = 0; s < splits; ++s)
+#pragma unroll
+                for (int h = 0; h < V / 4; ++h) {
+                    const f32x4 x = *(const f32x4*)(p + s * step + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[4 * h + j] += x[j];
+                }
         } else {
             for (int s = 0; s < splits; ++s)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (col + c < n) v[c] += p[(int64_t)s * m * n + c];
+                for (int j = 0; j < V; ++j)
+                    if (col + j < n) v[j] += p[s * step + j];
         }
-        epilogue4<E>(e, row, col, n, v);
+        Raw<E, V> res;
+        if (e.residual && e.whole) res = elem_load<E, V>(e.residual, row * e.r_ld + col);
+        finish<E, V>(e, row, col, n, bias, res, v);
     }
 }
 
@@ -325,7 +402,8 @@ struct DzArgs {
     float slope;
     const void *z, *dy;
     int64_t dy_ld;
-    void* dz;     // [rows, n] or NULL
+    void* dz;     // [rows, dz_ld] or NULL; columns n .. dz_ld - 1 are set to 0
+    int dz_ld;
     float* part;  // [gridDim.y, n] or NULL
 };
 
@@ -335,6 +413,8 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
     const int tx = threadIdx.x % a.tx, ty = threadIdx.x / a.tx, TY = 256 / a.tx;
     const int64_t c = ((int64_t)blockIdx.x * a.tx + tx) * V;
     const bool in = c < a.n;
+    if (!in && a.dz && c < a.dz_ld)  // (only element by element: V = 1)
+        for (int64_t r = (int64_t)blockIdx.y * TY + ty; r < a.rows; r += (int64_t)gridDim.y * TY) ((typename E::type*)a.dz)[r * a.dz_ld + c] = (typename E::type)0.f;
     float sum[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = 0.f;
@@ -353,7 +433,7 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += v[j];
-            if (a.dz) elem_store<E, V>(a.dz, r * a.n + c, v);
+            if (a.dz) elem_store<E, V>(a.dz, r * a.dz_ld + c, v);
         }
     }
     if (!a.part) return;
@@ -376,52 +456,107 @@ int by_type(int type, F f) {
     return f(ElemF16());
 }
 
-// ---- host -------------------------------------------------------------------------------------------------------------------------
-struct Operand_ { const void* p; int64_t ld; bool across; };
+// Copies of up to three matrices whose rows are not whole 16-byte pieces, filled up with zeros.  A workgroup takes rows in turn.
+struct CopyArgs {
+    const void* from[3];
+    void* to[3];
+    int64_t ld[3], rows[3];
+    int cols[3], wide[3];
+};
+template <class E>
+__global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
+    typedef typename E::type T;
+    const int q = blockIdx.y;
+    const T* from = (const T*)a.from[q];
+    T* to = (T*)a.to[q];
+    const int wide = a.wide[q], pieces = wide / E::vec;
+    const int64_t all = a.rows[q] * pieces;
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += (int64_t)gridDim.x * 256) {
+        const int64_t r = id / pieces;
+        const int c = (int)(id - r * pieces) * E::vec;
+        T x[E::vec];
+#pragma unroll
+        for (int j = 0; j < E::vec; ++j) x[j] = c + j < a.cols[q] ? from[r * a.ld[q] + c + j] : (T)0.f;
+        f32x4 v;
+        __builtin_memcpy(&v, x, 16);
+        *(f32x4*)(to + r * wide + c) = v;
+    }
+}
 
-bool pieces_ok(const Operand_& o, int64_t rows, int size) {
-    const int pe = 16 / size;
-    return aligned16(o.p) && o.ld % pe == 0 && (!o.across || rows % pe == 0);
+// ---- host -------------------------------------------------------------------------------------------------------------------------
+// A matrix as the products read it: rows of `cols` elements in whole 16-byte pieces (`wide` of them there to be read)
+struct Mat { const void* p; int64_t ld, rows; int cols, wide; };
+
+int wide_of(int cols, int size) { return gcp_round_up(cols, 16 / size); }
+bool in_pieces(const void* p, int64_t ld, int cols, int size) {
+    // (a stride so long that the offsets within a tile of 256 rows pass 32 bits is shortened by the copy, too)
+    return aligned16(p) && ld % (16 / size) == 0 && cols % (16 / size) == 0 && ld < (int64_t)1 << 21;
+}
+int64_t copy_floats(int64_t rows, int cols, int size) { return (rows * wide_of(cols, size) * size + 15) / 16 * 4; }
+
+// Gives every matrix that needs it a copy in `space`, which moves on behind them.
+template <class E>
+int put_in_pieces(Mat* const* mats, int n, float*& space, hipStream_t stream) {
+    constexpr int size = (int)sizeof(typename E::type);
+    CopyArgs a = {};
+    int count = 0;
+    int64_t most = 0;
+    for (int i = 0; i < n; ++i) {
+        Mat& x = *mats[i];
+        x.wide = x.cols;
+        if (x.rows == 0 || in_pieces(x.p, x.ld, x.cols, size)) continue;
+        if (!space) return GCPNET_E_BADARG;
+        a.from[count] = x.p; a.ld[count] = x.ld; a.rows[count] = x.rows; a.cols[count] = x.cols;
+        x.wide = wide_of(x.cols, size);
+        x.p = space; x.ld = x.wide;
+        a.to[count] = space; a.wide[count++] = x.wide;
+        space += copy_floats(x.rows, x.cols, size);
+        const int64_t blocks = (x.rows * (x.wide / E::vec) + 255) / 256;
+        most = blocks > most ? blocks : most;
+    }
+    if (!count) return 0;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(copy_kernel<E>), dim3((unsigned)(most < 2048 ? most : 2048), (unsigned)count), dim3(256), 0, stream, a);
+    GCP_HIP_CHECK_LAUNCH();
+    return 0;
 }
 
 template <class E, bool AC, bool BC>
 int launch_tiles(const Gemm& g, int shape, hipStream_t stream) {
     const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits);
-    switch (shape) {
-        case 0: hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2>), grid, dim3(256), 0, stream, g); break;
-        case 1: hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 2>), grid, dim3(256), 0, stream, g); break;
-        default: hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 256, 256, 2, 4>), grid, dim3(512), 0, stream, g); break;
-    }
+    if (shape == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2, 3>), grid, dim3(256), 0, stream, g);
+    else if (shape == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 2, 2>), grid, dim3(256), 0, stream, g);
+    else if constexpr (E::code != GCP_TYPE_F32) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 256, 256, 2, 4, 2>), grid, dim3(512), 0, stream, g);
     GCP_HIP_CHECK_LAUNCH();
     return 0;
 }
 
-// C = A B^T with the epilogue.  ws: gcp_linear_plan(m, n, k, size).floats of workspace.
+// C[m][n] = sum_k A[m][k] B[n][k] with the epilogue; A and B in pieces, as [m][k] and [n][k] or, across, [k][m] and [k][n].
+// ws: gcp_linear_plan(m, n, k, size).floats of workspace.
 template <class E>
-int product(int64_t m, int64_t n, int64_t k, Operand_ a, Operand_ b, const Epilogue& e, float* ws, hipStream_t stream) {
+int product(int64_t m, int64_t n, int64_t k, const Mat& a, bool a_across, const Mat& b, bool b_across, const Epilogue& e, float* ws, hipStream_t stream) {
     const GcpLinearPlan plan = gcp_linear_plan(m, n, k, (int)sizeof(typename E::type));
     if (plan.tiles_m > INT32_MAX / plan.tiles_n) return GCPNET_E_UNSUPPORTED;
     if (plan.splits > 1 && !ws) return GCPNET_E_BADARG;
     Gemm g = {};
     g.m = m; g.n = n; g.k = k;
     g.a = a.p; g.a_ld = a.ld; g.b = b.p; g.b_ld = b.ld;
-    g.a_fast = pieces_ok(a, m, (int)sizeof(typename E::type));
-    g.b_fast = pieces_ok(b, n, (int)sizeof(typename E::type));
+    g.a_rows = a_across ? a.wide : m;
+    g.b_rows = b_across ? b.wide : n;
     g.tiles_m = (int)plan.tiles_m; g.tiles_n = (int)plan.tiles_n; g.splits = plan.splits; g.k_per = plan.k_per;
     g.part = plan.splits > 1 ? ws : nullptr;
     g.e = e;
     int rc;
-    if (!a.across && !b.across) rc = launch_tiles<E, false, false>(g, plan.shape, stream);
-    else if (!a.across) rc = launch_tiles<E, false, true>(g, plan.shape, stream);
+    if (!a_across && !b_across) rc = launch_tiles<E, false, false>(g, plan.shape, stream);
+    else if (!a_across) rc = launch_tiles<E, false, true>(g, plan.shape, stream);
     else rc = launch_tiles<E, true, true>(g, plan.shape, stream);
     if (rc || plan.splits == 1) return rc;
-    const int64_t quads = m * ((n + 3) / 4), blocks = (quads + 255) / 256;
+    const int64_t vecs = m * ((n + E::vec - 1) / E::vec), blocks = (vecs + 255) / 256;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(join_kernel<E>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, g.part, plan.splits, m, n, e);
     GCP_HIP_CHECK_LAUNCH();
     return 0;
 }
 
-bool quads_ok(const void* p, int64_t ld, int size) { return ((uintptr_t)p & (4 * size - 1)) == 0 && ld % 4 == 0; }
+bool whole_rows(const void* p, int64_t ld, int size) { return aligned16(p) && ld % (16 / size) == 0; }
 
 constexpr int DZ_GROUPS = 256;
 
@@ -430,87 +565,103 @@ int check_desc(const gcp_linear_t* l) {
     if (l->bias_type != GCP_TYPE_F32 && l->bias_type != l->type) return GCPNET_E_BADARG;
     if (l->rows > 0 && (!l->x || l->x_ld < 0)) return GCPNET_E_BADARG;
     if (!l->w || l->w_ld < 0) return GCPNET_E_BADARG;
-    if (l->rows > INT32_MAX) return GCPNET_E_UNSUPPORTED;
+    if (l->rows > INT32_MAX || l->k >= 1 << 21 || l->n >= 1 << 21) return GCPNET_E_UNSUPPORTED;
     return 0;
 }
 
+int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }
+
 }  // namespace
 
-extern "C" int64_t gcpnet_linear_act_workspace(int64_t rows, int k, int n, int type, int backward) {
-    if (rows < 0 || k < 1 || n < 1 || !elem_type_ok(type)) return GCPNET_E_BADARG;
-    const int size = elem_bytes(type);
-    if (!backward) return gcp_linear_plan(rows, n, k, size).floats;
-    const int64_t a = gcp_linear_plan(rows, k, n, size).floats, b = gcp_linear_plan(n, k, rows, size).floats, c = (int64_t)DZ_GROUPS * n;
-    return a > b ? (a > c ? a : c) : (b > c ? b : c);
+extern "C" int64_t gcpnet_linear_act_workspace(const gcp_linear_t* l, int backward) {
+    if (int rc = check_desc(l)) return rc;
+    const int size = elem_bytes(l->type);
+    const int64_t rows = l->rows;
+    int64_t copies = 0;
+    if (rows > 0 && !in_pieces(l->x, l->x_ld, l->k, size)) copies += copy_floats(rows, l->k, size);
+    if (rows > 0 && !in_pieces(l->w, l->w_ld, l->k, size)) copies += copy_floats(l->n, l->k, size);
+    if (!backward) return copies + gcp_linear_plan(rows, l->n, l->k, size).floats;
+    copies += copy_floats(rows, l->n, size);  // dz, or a copy of dy
+    const int64_t parts = larger(gcp_linear_plan(rows, l->k, l->n, size).floats, gcp_linear_plan(l->n, l->k, rows, size).floats);
+    return copies + larger(parts, (int64_t)DZ_GROUPS * l->n);
 }
 
 extern "C" int gcpnet_linear_act_forward(const gcp_linear_t* l, const void* residual, int64_t r_ld, void* y, void* z, float* workspace, void* stream) {
     if (int rc = check_desc(l)) return rc;
     if (l->rows == 0) return 0;
-    if (!y || r_ld < 0) return GCPNET_E_BADARG;
+    if (!y || r_ld < 0 || !aligned16(workspace)) return GCPNET_E_BADARG;
     const int size = elem_bytes(l->type);
     Epilogue e = {};
     e.bias = l->bias; e.bias_f32 = l->bias_type == GCP_TYPE_F32;
     e.residual = residual; e.r_ld = r_ld;
     e.act = l->act; e.slope = l->slope;
     e.y = y; e.z = z;
-    e.whole = l->n % 4 == 0 && quads_ok(y, l->n, size) && quads_ok(z, l->n, size) && quads_ok(residual, r_ld, size);
+    e.whole = whole_rows(y, l->n, size) && whole_rows(z, l->n, size) && whole_rows(residual, r_ld, size);
     return by_type(l->type, [&](auto t) {
-        return product<decltype(t)>(l->rows, l->n, l->k, {l->x, l->x_ld, false}, {l->w, l->w_ld, false}, e, workspace, (hipStream_t)stream);
+        typedef decltype(t) E;
+        Mat x = {l->x, l->x_ld, l->rows, l->k, 0}, w = {l->w, l->w_ld, l->n, l->k, 0};
+        Mat* const both[2] = {&x, &w};
+        if (int rc = put_in_pieces<E>(both, 2, workspace, (hipStream_t)stream)) return rc;
+        return product<E>(l->rows, l->n, l->k, x, false, w, false, e, workspace, (hipStream_t)stream);
     });
 }
 
-extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, const void* dy, int64_t dy_ld, void* dz, void* dx, void* dw, void* db,
+extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, const void* dy, int64_t dy_ld, void* dx, void* dw, void* db,
                                           float* workspace, void* stream) {
     if (int rc = check_desc(l)) return rc;
     const bool act = l->act != GCP_ACT_NONE;
-    if (dy_ld < 0 || (l->rows > 0 && (!dy || (act && (!z || !dz))))) return GCPNET_E_BADARG;
+    if (dy_ld < 0 || (l->rows > 0 && (!dy || (act && !z))) || !aligned16(workspace)) return GCPNET_E_BADARG;
+    if ((db || (act && l->rows > 0)) && !workspace) return GCPNET_E_BADARG;
     const int size = elem_bytes(l->type);
     const hipStream_t st = (hipStream_t)stream;
-    const void* g = dy;  // the gradient of z
-    int64_t g_ld = dy_ld;
-    if (db || (act && l->rows > 0)) {
-        if (db && !workspace) return GCPNET_E_BADARG;
-        DzArgs a = {};
-        a.rows = l->rows; a.n = l->n; a.act = l->act; a.slope = l->slope;
-        a.z = z; a.dy = dy; a.dy_ld = dy_ld; a.dz = act ? dz : nullptr;
-        a.part = db ? workspace : nullptr;
-        const int v = 16 / size;
-        const bool vec = l->n % v == 0 && dy_ld % v == 0 && aligned16(dy) && (!act || (aligned16(z) && aligned16(dz)));
-        const int64_t across = vec ? l->n / v : l->n;
-        a.tx = 8;
-        while (a.tx < 256 && a.tx < across) a.tx *= 2;
-        const int64_t bx = (across + a.tx - 1) / a.tx, ty = 256 / a.tx;
-        // (two workgroups per CU in all; a thread takes eight rows or more before there are more groups of rows)
-        int64_t by = (l->rows + 8 * ty - 1) / (8 * ty), most = (512 + bx - 1) / bx;
-        by = by < most ? by : most;
-        by = by < DZ_GROUPS ? by : DZ_GROUPS;
-        if (by > 0) {
-            const int rc = by_type(l->type, [&](auto t) {
-                typedef decltype(t) E;
+    return by_type(l->type, [&](auto t) {
+        typedef decltype(t) E;
+        Mat x = {l->x, l->x_ld, l->rows, l->k, 0}, w = {l->w, l->w_ld, l->n, l->k, 0}, g = {dy, dy_ld, l->rows, l->n, 0};
+        Mat* mats[3];
+        int count = 0;
+        if (dw) mats[count++] = &x;
+        if (dx && l->rows > 0) mats[count++] = &w;
+        if (!act && (dw || dx)) mats[count++] = &g;
+        if (int rc = put_in_pieces<E>(mats, count, workspace, st)) return rc;
+        if (db || (act && l->rows > 0 && (dw || dx))) {
+            DzArgs a = {};
+            a.rows = l->rows; a.n = l->n; a.act = l->act; a.slope = l->slope;
+            a.z = z; a.dy = dy; a.dy_ld = dy_ld;
+            a.dz_ld = wide_of(l->n, size);
+            if (act && (dw || dx)) {
+                a.dz = workspace;
+                g.p = workspace; g.ld = g.wide = a.dz_ld;
+                workspace += copy_floats(l->rows, l->n, size);
+            }
+            a.part = db ? workspace : nullptr;
+            const int v = 16 / size;
+            const bool vec = l->n % v == 0 && dy_ld % v == 0 && aligned16(dy) && (!act || aligned16(z));
+            const int64_t across = vec ? l->n / v : a.dz ? a.dz_ld : l->n;
+            a.tx = 8;
+            while (a.tx < 256 && a.tx < across) a.tx *= 2;
+            const int64_t bx = (across + a.tx - 1) / a.tx, ty = 256 / a.tx;
+            // (two workgroups per CU in all; a thread takes eight rows or more before there are more groups of rows)
+            int64_t by = (l->rows + 8 * ty - 1) / (8 * ty), most = (512 + bx - 1) / bx;
+            by = by < most ? by : most;
+            by = by < DZ_GROUPS ? by : DZ_GROUPS;
+            if (by > 0) {
                 if (vec) hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<E, E::vec>), dim3((unsigned)bx, (unsigned)by), dim3(256), 0, st, a);
                 else hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<E, 1>), dim3((unsigned)bx, (unsigned)by), dim3(256), 0, st, a);
                 GCP_HIP_CHECK_LAUNCH();
-                return 0;
-            });
-            if (rc) return rc;
+            }
+            if (db)
+                if (const int rc = gcp_column_sums(workspace, (int)by, 1, l->n, &db, &l->bias_type, st)) return rc;
         }
-        if (db)
-            if (const int rc = gcp_column_sums(workspace, (int)by, 1, l->n, &db, &l->bias_type, st)) return rc;
-        if (act) { g = dz; g_ld = l->n; }
-    }
-    return by_type(l->type, [&](auto t) {
-        typedef decltype(t) E;
         Epilogue e = {};
         if (dx && l->rows > 0) {
             e.y = dx;
-            e.whole = l->k % 4 == 0 && quads_ok(dx, l->k, size);
-            if (int rc = product<E>(l->rows, l->k, l->n, {g, g_ld, false}, {l->w, l->w_ld, true}, e, workspace, st)) return rc;
+            e.whole = whole_rows(dx, l->k, size);
+            if (int rc = product<E>(l->rows, l->k, l->n, g, false, w, true, e, workspace, st)) return rc;
         }
         if (dw) {
             e.y = dw;
-            e.whole = l->k % 4 == 0 && quads_ok(dw, l->k, size);
-            if (int rc = product<E>(l->n, l->k, l->rows, {g, g_ld, true}, {l->x, l->x_ld, true}, e, workspace, st)) return rc;
+            e.whole = whole_rows(dw, l->k, size);
+            if (int rc = product<E>(l->n, l->k, l->rows, g, true, x, true, e, workspace, st)) return rc;
         }
         return 0;
     });

@@ -9,15 +9,16 @@ struct GcpLinearPlan {
     int64_t k_per, floats;  // k of a split; workspace
 };
 
-// The largest tile that still gives every CU (256) a workgroup: a large tile reads its operands fewer times, but idle CUs cost more.
-// With fewer workgroups than CUs even so, k is split, in pieces of at least eight tiles of 128 bytes.
+// The largest tile that still gives every CU (256) two workgroups: a large tile reads its operands fewer times, but idle CUs cost more.
+// With fewer workgroups than CUs even so, k is split, in pieces of at least eight tiles of 128 bytes.  (fp32 takes the matrix pipe 16
+// times as long per byte: 128 x 128 tiles feed it.)
 inline GcpLinearPlan gcp_linear_plan(int64_t m, int64_t n, int64_t k, int size) {
     const int64_t ke = 128 / size, steps = (k + ke - 1) / ke;
     GcpLinearPlan p = {};
-    for (p.shape = 2; p.shape >= 0; --p.shape) {
-        const int64_t b = 64 << p.shape;
-        p.tiles_m = (m + b - 1) / b;
-        p.tiles_n = (n + b - 1) / b;
+    for (p.shape = size == 4 ? 1 : 2; p.shape >= 0; --p.shape) {
+        const int64_t bm = 64 << p.shape, bn = bm;
+        p.tiles_m = (m + bm - 1) / bm;
+        p.tiles_n = (n + bn - 1) / bn;
         if (p.tiles_m * p.tiles_n >= 256 || p.shape == 0) break;
     }
     const int64_t tiles = p.tiles_m * p.tiles_n;

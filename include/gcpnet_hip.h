@@ -606,9 +606,9 @@ int gcpnet_adamw_step(int n, const gcp_adamw_tensor_t* tensors, int type, int st
 /* ---- Linear with its epilogue, forward and backward (fp32, bf16 or fp16; sums in fp32):
  *   z = x W^T + b;  y = act(z) + residual;   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz
  * x [rows, k], w [n, k], residual [rows, n], dy [rows, n] have unit column stride and any row stride; bias [n] of bias_type (fp32 or `type`) or
- * NULL; y, z, dz, dx, dw, db are contiguous, db of bias_type.  z (pre-activation, for the backward) may be NULL, without an activation it is not
- * needed.  dz is scratch [rows, n], needed with an activation; dx, dw, db may each be NULL.  workspace:
- * gcpnet_linear_act_workspace(...) floats (16-byte aligned; NULL where that is 0). */
+ * NULL; y, z, dx, dw, db are contiguous, db of bias_type; k, n < 2^21.  z (pre-activation, for the backward) may be NULL, without an activation
+ * it is not needed.  dx, dw, db may each be NULL.  workspace: gcpnet_linear_act_workspace(l, ...) floats (16-byte aligned; NULL where that is 0),
+ * which go by the descriptor as it is then passed. */
 typedef struct {
     int64_t rows;
     int k, n, type, bias_type, act;
@@ -616,9 +616,9 @@ typedef struct {
     const void *x, *w, *bias;
     int64_t x_ld, w_ld;
 } gcp_linear_t;
-int64_t gcpnet_linear_act_workspace(int64_t rows, int k, int n, int type, int backward);
+int64_t gcpnet_linear_act_workspace(const gcp_linear_t* l, int backward);
 int gcpnet_linear_act_forward(const gcp_linear_t* l, const void* residual, int64_t r_ld, void* y, void* z, float* workspace, void* stream);
-int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, const void* dy, int64_t dy_ld, void* dz, void* dx, void* dw, void* db,
+int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, const void* dy, int64_t dy_ld, void* dx, void* dw, void* db,
                                float* workspace, void* stream);
 
 /* ---- norms before and after a residual block with its gate and residual scale (fp32, bf16 or fp16 rows; everything in between in fp32):

@@ -284,16 +284,21 @@ def test_refusals():
     call = lambda y=None: lib.gcpnet_linear_act_forward(q, None, 0, y, None, None, None)  # noqa: E731
     assert call() == -1  # (no y)
     for field, bad, code in (("k", 0, -1), ("n", 0, -1), ("rows", -1, -1), ("type", 3, -1), ("bias_type", 2, -1), ("act", 6, -1), ("x", None, -1),
-                             ("w", None, -1), ("x_ld", -1, -1), ("rows", 1 << 33, -2)):
+                             ("w", None, -1), ("x_ld", -1, -1), ("rows", 1 << 33, -2), ("k", 1 << 21, -2), ("n", 1 << 21, -2)):
         keep = getattr(q, field)
         setattr(q, field, bad)
         assert call(4096) == code, field
         setattr(q, field, keep)
     q.act = 4
-    assert lib.gcpnet_linear_act_backward(q, None, 4096, 12, None, None, None, None, None, None) == -1  # (no z)
+    assert lib.gcpnet_linear_act_backward(q, None, 4096, 12, None, None, None, None, None) == -1  # (no z)
     q.act = 0
-    assert lib.gcpnet_linear_act_backward(q, None, 4096, 12, None, None, None, 4096, None, None) == -1  # (db without workspace)
-    assert lib.gcpnet_linear_act_workspace(4, 8, 12, 7, 0) == -1
+    assert lib.gcpnet_linear_act_backward(q, None, 4096, 12, None, None, 4096, None, None) == -1  # (db without workspace)
+    assert lib.gcpnet_linear_act_workspace(q, 0) == 0 and lib.gcpnet_linear_act_forward(q, None, 0, 4096, None, 8, None) == -1  # (off 16 bytes)
+    q.x = 4098  # (its copy: 4 rows of 8 floats; in a backward dz and the column sums of 256 groups too)
+    assert lib.gcpnet_linear_act_workspace(q, 0) == 32 and lib.gcpnet_linear_act_workspace(q, 1) == 32 + 48 + 256 * 12
+    q.type = 7
+    assert lib.gcpnet_linear_act_workspace(q, 0) == -1
+    q.type = 0
     q.rows = 0
     assert call() == 0
 
