@@ -129,7 +129,7 @@ def _norm_backward(ctx, ds, dh):
             dws[i] = v
     scratch = None
     if wanted or (dgate is not None and ctx.channel):
-        scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(n.rows, n.d))), dtype=torch.float32, device=s.device)
+        scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(C.byref(b)))), dtype=torch.float32, device=s.device)
     check(lib.gcpnet_block_norm_backward(C.byref(b), s.data_ptr(), _ptr(stats), _ptr(ds), _ptr(dh), _ptr(dx), _ptr(dy), _ptr(dgate),
                                          *map(_ptr, dws), _ptr(scratch), _stream()), "residual_norm backward")
     return (None, dx, dy, dgate, *dws)

@@ -7,55 +7,104 @@ struct ElemBf16 { typedef __bf16 type; static constexpr int code = GCP_TYPE_BF16
 struct ElemF16 { typedef _Float16 type; static constexpr int code = GCP_TYPE_F16, vec = 8; };
 
 template <class E, int V>
-struct Raw {  // V elements, loaded and stored as one piece (V = 1 or 16 bytes' worth)
-    typename E::type x[V];
-    static constexpr int bytes = V * (int)sizeof(typename E::type);
+struct Raw {  // V elements as they lie in memory, 16 bytes in four registers
+    unsigned u[4];
+    __device__ __forceinline__ float operator[](int j) const {
+        if constexpr (E::code == GCP_TYPE_F32) return __uint_as_float(u[j]);
+        else if constexpr (E::code == GCP_TYPE_BF16) return __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
+        else return (float)__builtin_bit_cast(_Float16, (unsigned short)(j & 1 ? u[j / 2] >> 16 : u[j / 2]));
+    }
 };
 
+// Loads and stores of V elements at any element's address: one 16-byte access (global memory takes it at any alignment), and element by
+// element where only the first `count` of the V are there.
 template <class E, int V>
 __device__ __forceinline__ Raw<E, V> elem_load(const void* base, int64_t at) {
+    static_assert(V * sizeof(typename E::type) == 16, "a vector is 16 bytes");
     Raw<E, V> r;
-    const typename E::type* p = (const typename E::type*)base + at;
-    if constexpr (V == 1) {
-        r.x[0] = *p;
-    } else {
-        static_assert(Raw<E, V>::bytes == 16, "a vector is 16 bytes");
-        const f32x4 q = *(const f32x4*)p;
-        __builtin_memcpy(r.x, &q, 16);
-    }
+    __builtin_memcpy(r.u, (const typename E::type*)base + at, 16);
+    return r;
+}
+template <class E, int V>
+__device__ __forceinline__ Raw<E, V> elem_zero() {
+    return Raw<E, V>{{0u, 0u, 0u, 0u}};
+}
+template <class E, int V>
+__device__ __forceinline__ Raw<E, V> elem_load(const void* base, int64_t at, int count) {
+    if (count == V) return elem_load<E, V>(base, at);
+    Raw<E, V> r = elem_zero<E, V>();
+    if (count > 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < count) {
+                if constexpr (E::code == GCP_TYPE_F32) r.u[j] = ((const unsigned*)base)[at + j];
+                else r.u[j / 2] |= (unsigned)((const unsigned short*)base)[at + j] << (16 * (j & 1));
+            }
     return r;
 }
 template <class E, int V>
 __device__ __forceinline__ void elem_store(void* base, int64_t at, const float (&f)[V]) {
-    typename E::type* p = (typename E::type*)base + at;
-    if constexpr (V == 1) {
-        *p = (typename E::type)f[0];
-    } else {
-        typename E::type x[V];
+    typename E::type x[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = (typename E::type)f[j];  // (nearest even)
-        f32x4 q;
-        __builtin_memcpy(&q, x, 16);
-        *(f32x4*)p = q;
-    }
+    for (int j = 0; j < V; ++j) x[j] = (typename E::type)f[j];  // (nearest even)
+    f32x4 q;
+    __builtin_memcpy(&q, x, 16);
+    __builtin_memcpy((typename E::type*)base + at, &q, 16);
 }
 template <class E, int V>
-__device__ __forceinline__ void elem_zero(Raw<E, V>& r) {
+__device__ __forceinline__ void elem_store(void* base, int64_t at, const float (&f)[V], int count) {
+    if (count == V) elem_store<E, V>(base, at, f);
+    else if (count > 0)
 #pragma unroll
-    for (int j = 0; j < V; ++j) r.x[j] = (typename E::type)0.f;
+        for (int j = 0; j < V; ++j)
+            if (j < count) ((typename E::type*)base)[at + j] = (typename E::type)f[j];
 }
 
-// V values of a parameter vector of the same type as the rows, or fp32 (`f32`: uniform over the launch)
+// `count` of V values of a parameter vector of the rows' type, or fp32 (`f32`: uniform over the launch); without one they stay as they are
 template <class E, int V>
-__device__ __forceinline__ void param_load(const void* base, int64_t at, bool f32, float (&f)[V]) {
-    if (!base) return;
+__device__ __forceinline__ void param_load(const void* base, int64_t at, int count, bool f32, float (&f)[V]) {
+    if (!base || count <= 0) return;
     if (E::code != GCP_TYPE_F32 && f32) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = ((const float*)base)[at + j];
-    } else {
-        const Raw<E, V> r = elem_load<E, V>(base, at);
+        for (int h = 0; h < V; h += 4) {
+            const Raw<ElemF32, 4> r = elem_load<ElemF32, 4>(base, at + h, count - h < 4 ? count - h : 4);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = (float)r.x[j];
+            for (int j = 0; j < 4; ++j) f[h + j] = r[j];
+        }
+    } else {
+        const Raw<E, V> r = elem_load<E, V>(base, at, count);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = r[j];
+    }
+}
+
+// act(v), and with GRAD also act'(v), of V values; the choice is uniform and made once for all of them.  The sigmoid's reciprocal is the
+// hardware's, good to a unit in the last place of fp32.
+template <int V, bool GRAD>
+__device__ __forceinline__ void elem_act(int act, float slope, const float (&v)[V], float (&a)[V], float (&d)[V]) {
+    if (act == GCP_ACT_SILU || act == GCP_ACT_SIGMOID) {
+        const bool silu = act == GCP_ACT_SILU;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float x = v[j], s = __builtin_amdgcn_rcpf(1.f + __expf(-x)), r = s * (1.f - s);
+            a[j] = silu ? x * s : s;
+            if constexpr (GRAD) d[j] = silu ? fmaf(x, r, s) : r;
+        }
+    } else if (act == GCP_ACT_SELU) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float x = v[j];
+            a[j] = gcp_act(GCP_ACT_SELU, x, slope);
+            if constexpr (GRAD) d[j] = gcp_act_grad(GCP_ACT_SELU, x, slope);
+        }
+    } else {  // (none, relu, leakyrelu: a slope on each side)
+        const float low = act == GCP_ACT_NONE ? 1.f : act == GCP_ACT_RELU ? 0.f : slope;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float x = v[j];
+            a[j] = x > 0.f || act == GCP_ACT_NONE ? x : (low == 0.f ? 0.f : low * x);
+            if constexpr (GRAD) d[j] = x > 0.f ? 1.f : low;
+        }
     }
 }
 

@@ -36,7 +36,7 @@ constexpr int KROW = 128;  // bytes of k in a tile
 struct Epilogue {
     const void *bias, *residual;
     int64_t r_ld;
-    int act, bias_f32, whole;  // whole: 16 bytes at a time (all rows of y, z, residual allow it)
+    int act, bias_f32;
     float slope;
     void *y, *z;  // contiguous [m, n]
 };
@@ -52,63 +52,26 @@ struct Gemm {
     Epilogue e;
 };
 
-// act of V values; the choice is uniform and made once for all of them.  (The reciprocal is good to a unit in the last place of fp32.)
-template <int V>
-__device__ __forceinline__ void act_all(int act, float slope, float (&v)[V]) {
-    if (act == GCP_ACT_NONE) return;
-    if (act == GCP_ACT_RELU || act == GCP_ACT_LEAKYRELU) {
-        const float low = act == GCP_ACT_RELU ? 0.f : slope;
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = v[j] > 0.f ? v[j] : (low == 0.f ? 0.f : low * v[j]);
-    } else if (act == GCP_ACT_SELU) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = gcp_act(GCP_ACT_SELU, v[j], slope);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-v[j]));
-            v[j] = act == GCP_ACT_SILU ? v[j] * s : s;
-        }
-    }
-}
-
-// V columns of one row from n on: bias, z, activation, residual (`r`, loaded before, where the rows are whole), y
+// V columns of one row from n on, `count` of them there: bias, z, activation, residual (`r`, loaded before), y
 template <class E, int V>
-__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, int64_t N, const float (&bias)[V], const Raw<E, V>& r, float (&v)[V]) {
-    typedef typename E::type T;
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, int64_t N, int count, const float (&bias)[V], const Raw<E, V>& r, float (&v)[V]) {
     const int64_t at = m * N + n;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += bias[j];
-    if (e.whole) {
-        if (e.z) elem_store<E, V>(e.z, at, v);
-        act_all<V>(e.act, e.slope, v);
-        if (e.residual)
+    if (e.z) elem_store<E, V>(e.z, at, v, count);
+    float none[V];
+    elem_act<V, false>(e.act, e.slope, v, v, none);
+    if (e.residual)
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] += (float)r.x[j];
-        elem_store<E, V>(e.y, at, v);
-    } else {
-        if (e.z)
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (n + j < N) ((T*)e.z)[at + j] = (T)v[j];
-        act_all<V>(e.act, e.slope, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (n + j < N) {
-                if (e.residual) v[j] += (float)((const T*)e.residual)[m * e.r_ld + n + j];
-                ((T*)e.y)[at + j] = (T)v[j];
-            }
-    }
+        for (int j = 0; j < V; ++j) v[j] += r[j];
+    elem_store<E, V>(e.y, at, v, count);
 }
 
 template <class E, int V>
-__device__ __forceinline__ void bias_load(const Epilogue& e, int64_t n, int64_t N, float (&bias)[V]) {
+__device__ __forceinline__ void bias_load(const Epilogue& e, int64_t n, int count, float (&bias)[V]) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        bias[j] = 0.f;
-        if (e.bias && n + j < N)
-            bias[j] = (E::code != GCP_TYPE_F32 && e.bias_f32) ? ((const float*)e.bias)[n + j] : (float)((const typename E::type*)e.bias)[n + j];
-    }
+    for (int j = 0; j < V; ++j) bias[j] = 0.f;
+    param_load<E, V>(e.bias, n, count, e.bias_f32, bias);
 }
 
 // 16 bytes per lane from memory (uniform base + offset) to LDS (lane l to base + 16 l), counted by vmcnt.  In asm, because the compiler would
@@ -308,8 +271,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
     static_assert(PH >= 16 && ROWS % PH == 0 && PH % (RPP * AT_ONCE) == 0, "whole phases");
     f32x4* own = (f32x4*)(lds + wave * OWN);
     const int64_t n = n0 + wn * COLS + (lane % LPR) * V;
+    const int count = g.n - n < V ? (int)(g.n - n) : V;
     float bias[V];
-    bias_load<E, V>(g.e, n, g.n, bias);
+    bias_load<E, V>(g.e, n, count, bias);
 #pragma unroll
     for (int ph = 0; ph < ROWS / PH; ++ph) {
         gcp_wave_lds_sync();  // (lanes exchange: what the phase before read has been read)
@@ -325,11 +289,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
         for (int r0 = 0; r0 < PH; r0 += RPP * AT_ONCE) {
             // (the residual of several passes is requested before the first is finished)
             Raw<E, V> res[AT_ONCE];
-            if (g.e.residual && g.e.whole && !g.part)
+            if (g.e.residual && !g.part)
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u) {
                     const int64_t m = m0 + wm * ROWS + ph * PH + r0 + u * RPP + lane / LPR;
-                    if (m < g.m && n < g.n) res[u] = elem_load<E, V>(g.e.residual, m * g.e.r_ld + n);
+                    if (m < g.m) res[u] = elem_load<E, V>(g.e.residual, m * g.e.r_ld + n, count);
                 }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
@@ -342,19 +306,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
                 }
-                if (m >= g.m || n >= g.n) continue;
+                if (m >= g.m || count <= 0) continue;
                 if (g.part) {
-                    float* p = g.part + ((int64_t)blockIdx.y * g.m + m) * g.n + n;
-                    if (g.n % V == 0) {
 #pragma unroll
-                        for (int h = 0; h < V / 4; ++h) *(f32x4*)(p + 4 * h) = f32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < V; ++j)
-                            if (n + j < g.n) p[j] = v[j];
+                    for (int h = 0; h < V; h += 4) {
+                        const float four[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+                        elem_store<ElemF32, 4>(g.part, ((int64_t)blockIdx.y * g.m + m) * g.n + n + h, four, count - h < 4 ? count - h : 4);
                     }
                 } else {
-                    finish<E, V>(g.e, m, n, g.n, bias, res[u], v);
+                    finish<E, V>(g.e, m, n, g.n, count, bias, res[u], v);
                 }
             }
         }
@@ -368,29 +328,22 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     const int64_t vecs = (n + V - 1) / V, all = m * vecs, step = m * n;
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += (int64_t)gridDim.x * 256) {
         const int64_t row = id / vecs, col = (id - row * vecs) * V;
+        const int count = n - col < V ? (int)(n - col) : V;
         float v[V], bias[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = 0.f;
-        const float* p = part + row * n + col;
-        bias_load<E, V>(e, col, n, bias);
-        if (n % V == 0) {
-#pragma unroll 4
-            for (int s = 0; s < splits; ++s)
-#pragma unroll
-                for (int h = 0; h < V / 4; ++h) {
-                    const f32x4 x = *(const f32x4*)(p + s * step + 4 * h);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[4 * h + j] += x[j];
-                }
-        } else {
-            for (int s = 0; s < splits; ++s)
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (col + j < n) v[j] += p[s * step + j];
-        }
+        bias_load<E, V>(e, col, count, bias);
         Raw<E, V> res;
-        if (e.residual && e.whole) res = elem_load<E, V>(e.residual, row * e.r_ld + col);
-        finish<E, V>(e, row, col, n, bias, res, v);
+        if (e.residual) res = elem_load<E, V>(e.residual, row * e.r_ld + col, count);
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s)
+#pragma unroll
+            for (int h = 0; h < V; h += 4) {
+                const Raw<ElemF32, 4> x = elem_load<ElemF32, 4>(part, s * step + row * n + col + h, count - h < 4 ? count - h : 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[h + j] += x[j];
+            }
+        finish<E, V>(e, row, col, n, count, bias, res, v);
     }
 }
 
@@ -402,50 +355,55 @@ struct DzArgs {
     float slope;
     const void *z, *dy;
     int64_t dy_ld;
-    void* dz;     // [rows, dz_ld] or NULL; columns n .. dz_ld - 1 are set to 0
+    void* dz;     // [rows, dz_ld] or NULL; dz_ld: n rounded up to whole pieces, which are filled up with zeros
     int dz_ld;
     float* part;  // [gridDim.y, n] or NULL
 };
 
-template <class E, int V>
+template <class E>
 __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
+    constexpr int V = E::vec;
     __shared__ float cols[256 * V];
     const int tx = threadIdx.x % a.tx, ty = threadIdx.x / a.tx, TY = 256 / a.tx;
     const int64_t c = ((int64_t)blockIdx.x * a.tx + tx) * V;
-    const bool in = c < a.n;
-    if (!in && a.dz && c < a.dz_ld)  // (only element by element: V = 1)
-        for (int64_t r = (int64_t)blockIdx.y * TY + ty; r < a.rows; r += (int64_t)gridDim.y * TY) ((typename E::type*)a.dz)[r * a.dz_ld + c] = (typename E::type)0.f;
+    const int count = a.n - c < V ? (int)(a.n - c) : V;  // (0 or less: nothing to do)
     float sum[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = 0.f;
-    if (in) {
+    if (count > 0) {
 #pragma unroll 4
         for (int64_t r = (int64_t)blockIdx.y * TY + ty; r < a.rows; r += (int64_t)gridDim.y * TY) {
-            const Raw<E, V> dy = elem_load<E, V>(a.dy, r * a.dy_ld + c);
+            const Raw<E, V> dy = elem_load<E, V>(a.dy, r * a.dy_ld + c, count);
             float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = dy[j];
             if (a.act != GCP_ACT_NONE) {
-                const Raw<E, V> z = elem_load<E, V>(a.z, r * a.n + c);
+                const Raw<E, V> zr = elem_load<E, V>(a.z, r * a.n + c, count);
+                float z[V], act[V], d[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = (float)dy.x[j] * gcp_act_grad(a.act, (float)z.x[j], a.slope);
-            } else {
+                for (int j = 0; j < V; ++j) z[j] = zr[j];
+                elem_act<V, true>(a.act, a.slope, z, act, d);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = (float)dy.x[j];
+                for (int j = 0; j < V; ++j) v[j] = j < count ? v[j] * d[j] : 0.f;
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += v[j];
-            if (a.dz) elem_store<E, V>(a.dz, r * a.dz_ld + c, v);
+            if (a.dz) elem_store<E, V>(a.dz, r * a.dz_ld + c, v);  // (whole pieces: dz_ld is a multiple of them)
         }
     }
     if (!a.part) return;
 #pragma unroll
     for (int j = 0; j < V; ++j) cols[threadIdx.x * V + j] = sum[j];
     __syncthreads();
-    if (ty == 0 && in) {
+    if (ty == 0 && count > 0) {
         for (int y = 1; y < TY; ++y)
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += cols[(y * a.tx + tx) * V + j];
 #pragma unroll
-        for (int j = 0; j < V; ++j) a.part[(int64_t)blockIdx.y * a.n + c + j] = sum[j];
+        for (int h = 0; h < V; h += 4) {
+            const float four[4] = {sum[h], sum[h + 1], sum[h + 2], sum[h + 3]};
+            elem_store<ElemF32, 4>(a.part, (int64_t)blockIdx.y * a.n + c + h, four, count - h < 4 ? count - h : 4);
+        }
     }
 }
 
@@ -474,12 +432,8 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += (int64_t)gridDim.x * 256) {
         const int64_t r = id / pieces;
         const int c = (int)(id - r * pieces) * E::vec;
-        T x[E::vec];
-#pragma unroll
-        for (int j = 0; j < E::vec; ++j) x[j] = c + j < a.cols[q] ? from[r * a.ld[q] + c + j] : (T)0.f;
-        f32x4 v;
-        __builtin_memcpy(&v, x, 16);
-        *(f32x4*)(to + r * wide + c) = v;
+        const Raw<E, E::vec> x = elem_load<E, E::vec>(from, r * a.ld[q] + c, a.cols[q] - c < E::vec ? a.cols[q] - c : E::vec);
+        __builtin_memcpy(to + r * wide + c, x.u, 16);
     }
 }
 
@@ -556,8 +510,6 @@ int product(int64_t m, int64_t n, int64_t k, const Mat& a, bool a_across, const 
     return 0;
 }
 
-bool whole_rows(const void* p, int64_t ld, int size) { return aligned16(p) && ld % (16 / size) == 0; }
-
 constexpr int DZ_GROUPS = 256;
 
 int check_desc(const gcp_linear_t* l) {
@@ -590,13 +542,11 @@ extern "C" int gcpnet_linear_act_forward(const gcp_linear_t* l, const void* resi
     if (int rc = check_desc(l)) return rc;
     if (l->rows == 0) return 0;
     if (!y || r_ld < 0 || !aligned16(workspace)) return GCPNET_E_BADARG;
-    const int size = elem_bytes(l->type);
     Epilogue e = {};
     e.bias = l->bias; e.bias_f32 = l->bias_type == GCP_TYPE_F32;
     e.residual = residual; e.r_ld = r_ld;
     e.act = l->act; e.slope = l->slope;
     e.y = y; e.z = z;
-    e.whole = whole_rows(y, l->n, size) && whole_rows(z, l->n, size) && whole_rows(residual, r_ld, size);
     return by_type(l->type, [&](auto t) {
         typedef decltype(t) E;
         Mat x = {l->x, l->x_ld, l->rows, l->k, 0}, w = {l->w, l->w_ld, l->n, l->k, 0};
@@ -634,9 +584,7 @@ extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, 
                 workspace += copy_floats(l->rows, l->n, size);
             }
             a.part = db ? workspace : nullptr;
-            const int v = 16 / size;
-            const bool vec = l->n % v == 0 && dy_ld % v == 0 && aligned16(dy) && (!act || aligned16(z));
-            const int64_t across = vec ? l->n / v : a.dz ? a.dz_ld : l->n;
+            const int64_t across = a.dz_ld / E::vec;
             a.tx = 8;
             while (a.tx < 256 && a.tx < across) a.tx *= 2;
             const int64_t bx = (across + a.tx - 1) / a.tx, ty = 256 / a.tx;
@@ -645,8 +593,7 @@ extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, 
             by = by < most ? by : most;
             by = by < DZ_GROUPS ? by : DZ_GROUPS;
             if (by > 0) {
-                if (vec) hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<E, E::vec>), dim3((unsigned)bx, (unsigned)by), dim3(256), 0, st, a);
-                else hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<E, 1>), dim3((unsigned)bx, (unsigned)by), dim3(256), 0, st, a);
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<E>), dim3((unsigned)bx, (unsigned)by), dim3(256), 0, st, a);
                 GCP_HIP_CHECK_LAUNCH();
             }
             if (db)
@@ -655,12 +602,10 @@ extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, 
         Epilogue e = {};
         if (dx && l->rows > 0) {
             e.y = dx;
-            e.whole = whole_rows(dx, l->k, size);
             if (int rc = product<E>(l->rows, l->k, l->n, g, false, w, true, e, workspace, st)) return rc;
         }
         if (dw) {
             e.y = dw;
-            e.whole = whole_rows(dw, l->k, size);
             if (int rc = product<E>(l->n, l->k, l->rows, g, true, x, true, e, workspace, st)) return rc;
         }
         return 0;

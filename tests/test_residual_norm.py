@@ -366,7 +366,8 @@ def test_refusals():
     assert lib.gcpnet_block_norm_backward(n, 4096, None, *[None] * 11) == -1  # (pre without statistics)
     n.rows = 0
     assert call() == 0
-    assert lib.gcpnet_block_norm_backward_scratch(-1, 8) == -1
+    n.rows = -1
+    assert lib.gcpnet_block_norm_backward_scratch(n) == -1
 
 
 @pytest.mark.gpu
