@@ -14,6 +14,7 @@
 //     read, fp32 ones element by element;
 //   * operands whose rows are not whole 16-byte pieces are first copied into the workspace, rows filled up with zeros (one launch for all of
 //     them); where k ends inside a tile, the places behind it are set to zero;
+//   * a forward with few rows reads W once, straight into registers (few_rows_kernel);
 //   * few tiles of C: k is split over workgroups, which leave fp32 partial sums for a second launch that adds them in a fixed order and
 //     applies the epilogue (no atomics: results repeat bit for bit).
 // The epilogue adds the bias, applies the activation, adds the residual and rounds once; in training it also stores z.  The accumulators go
@@ -347,6 +348,76 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     }
 }
 
+static_assert(GCP_FEW_ROWS == 32, "two forms of few_rows_kernel");
+// Few rows (up to 16 MT): bound by the read of W, which goes from memory straight into the fragments of the matrix instructions, 512
+// consecutive bytes of each of 16 rows per wave and turn (4 rows, 4096 -> 8192 bf16: 14.6 us, 4.6 TB/s).  A workgroup takes 16 columns of y, its eight waves take turns along k; their sums
+// meet in LDS.  x comes from the caches.  Loads at any alignment: nothing is copied.
+struct FewRows {
+    int rows, k, n;
+    const void *x, *w;
+    int64_t x_ld, w_ld;
+    Epilogue e;
+};
+
+template <class E, int MT>
+__global__ __launch_bounds__(512) void few_rows_kernel(FewRows a) {
+    typedef typename E::type T;
+    constexpr int PE = 16 / (int)sizeof(T), U = 8, WAVES = 8, STEP = 4 * PE;  // k of one fragment
+    __shared__ f32x4 part[WAVES][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, row = n0 + i < a.n ? n0 + i : a.n - 1;  // (past the end: the last row again, not stored)
+    const T* w = (const T*)a.w + row * a.w_ld + q * PE;
+    const T* x[MT];
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = t * 16 + i < a.rows ? t * 16 + i : a.rows - 1;
+        x[t] = (const T*)a.x + m * a.x_ld + q * PE;
+        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int k = wave * U * STEP; k < a.k; k += WAVES * U * STEP) {
+        Raw<E, PE> fw[U];
+        if (k + U * STEP <= a.k) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) fw[u] = elem_load<E, PE>(w, k + u * STEP);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const Raw<E, PE> fx = elem_load<E, PE>(x[t], k + u * STEP);
+                    acc[t] = mfma<E>(__builtin_bit_cast(u32x4, fw[u]), __builtin_bit_cast(u32x4, fx), acc[t]);
+                }
+        } else {
+            for (int u = 0; u < U; ++u) {
+                const int left = a.k - (k + u * STEP + q * PE), count = left < 0 ? 0 : left < PE ? left : PE;
+                const Raw<E, PE> f = elem_load<E, PE>(w, k + u * STEP, count);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const Raw<E, PE> fx = elem_load<E, PE>(x[t], k + u * STEP, count);
+                    acc[t] = mfma<E>(__builtin_bit_cast(u32x4, f), __builtin_bit_cast(u32x4, fx), acc[t]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][i * 4 + q] = acc[t];  // (a lane: columns 4 q .. + 3 of row i)
+    __syncthreads();
+    for (int id = threadIdx.x; id < MT * 256; id += 512) {
+        const int t = id >> 8, r = id >> 4 & 15, c = id & 15, m = t * 16 + r, n = n0 + c;
+        if (m >= a.rows || n >= a.n) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int y = 0; y < WAVES; ++y) v += ((const float*)part[y][t])[r * 16 + c];
+        if (a.e.bias) v += (E::code != GCP_TYPE_F32 && a.e.bias_f32) ? ((const float*)a.e.bias)[n] : (float)((const T*)a.e.bias)[n];
+        const int64_t at = (int64_t)m * a.n + n;
+        if (a.e.z) ((T*)a.e.z)[at] = (T)v;
+        float one[1] = {v}, none[1];
+        elem_act<1, false>(a.e.act, a.e.slope, one, one, none);
+        if (a.e.residual) one[0] += (float)((const T*)a.e.residual)[m * a.e.r_ld + n];
+        ((T*)a.e.y)[at] = (T)one[0];
+    }
+}
+
 // dz = dy act'(z) (rounded to the rows' type: the matrix pipe takes 16-bit operands) and the partial column sums of the unrounded dz.
 // Threads of a workgroup: TX over vectors of columns, 256 / TX over rows; the rows of a workgroup are every gridDim.y-th group of them.
 struct DzArgs {
@@ -477,8 +548,14 @@ int put_in_pieces(Mat* const* mats, int n, float*& space, hipStream_t stream) {
 template <class E, bool AC, bool BC>
 int launch_tiles(const Gemm& g, int shape, hipStream_t stream) {
     const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits);
-    if (shape == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2, 3>), grid, dim3(256), 0, stream, g);
-    else if (shape == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 2, 2>), grid, dim3(256), 0, stream, g);
+    const int64_t groups = (int64_t)grid.x * grid.y;
+    // A longer ring hides more of the memory's latency, a shorter one lets more workgroups reside: few of them take the longer (2048^3 bf16, 256
+    // tiles of 128: 23.3 us with three, 26.4 with two; 500 x 4096 x 4096, 512 tiles of 64: 30.7 us with four, 36.0 with two; 3000 x 500 x 2001,
+    // 384 tiles of 128: 25.9 us with three, 22.9 with two; 2048^3 in 1024 tiles of 64: 35.0 with four, 27.2 with two).
+    if (shape == 0 && groups <= 512) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2, 4>), grid, dim3(256), 0, stream, g);
+    else if (shape == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2, 2>), grid, dim3(256), 0, stream, g);
+    else if (shape == 1 && groups <= 256) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 4, 3>), grid, dim3(512), 0, stream, g);
+    else if (shape == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 4, 2>), grid, dim3(512), 0, stream, g);
     else if constexpr (E::code != GCP_TYPE_F32) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 256, 256, 2, 4, 2>), grid, dim3(512), 0, stream, g);
     GCP_HIP_CHECK_LAUNCH();
     return 0;
@@ -530,6 +607,7 @@ extern "C" int64_t gcpnet_linear_act_workspace(const gcp_linear_t* l, int backwa
     const int size = elem_bytes(l->type);
     const int64_t rows = l->rows;
     int64_t copies = 0;
+    if (!backward && rows <= GCP_FEW_ROWS) return 0;
     if (rows > 0 && !in_pieces(l->x, l->x_ld, l->k, size)) copies += copy_floats(rows, l->k, size);
     if (rows > 0 && !in_pieces(l->w, l->w_ld, l->k, size)) copies += copy_floats(l->n, l->k, size);
     if (!backward) return copies + gcp_linear_plan(rows, l->n, l->k, size).floats;
@@ -549,6 +627,14 @@ extern "C" int gcpnet_linear_act_forward(const gcp_linear_t* l, const void* resi
     e.y = y; e.z = z;
     return by_type(l->type, [&](auto t) {
         typedef decltype(t) E;
+        if (l->rows <= GCP_FEW_ROWS) {
+            const FewRows f = {(int)l->rows, l->k, l->n, l->x, l->w, l->x_ld, l->w_ld, e};
+            const dim3 grid((unsigned)gcp_cdiv(l->n, 16));
+            if (l->rows <= 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<E, 1>), grid, dim3(512), 0, (hipStream_t)stream, f);
+            else hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<E, 2>), grid, dim3(512), 0, (hipStream_t)stream, f);
+            GCP_HIP_CHECK_LAUNCH();
+            return 0;
+        }
         Mat x = {l->x, l->x_ld, l->rows, l->k, 0}, w = {l->w, l->w_ld, l->n, l->k, 0};
         Mat* const both[2] = {&x, &w};
         if (int rc = put_in_pieces<E>(both, 2, workspace, (hipStream_t)stream)) return rc;

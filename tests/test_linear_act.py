@@ -107,7 +107,7 @@ def both_ways(x, w, b, act, r, dy, what=""):
     return out
 
 
-SHAPES = [(1, 1, 1), (1, 64, 64), (2, 3, 5), (3, 100, 200), (4, 512, 768), (7, 33, 130), (16, 100, 200), (17, 257, 31), (33, 64, 65), (64, 128, 64),
+SHAPES = [(1, 1, 1), (1, 64, 64), (2, 3, 5), (3, 100, 200), (4, 512, 768), (7, 33, 130), (16, 100, 200), (16, 1031, 48), (17, 257, 31), (32, 2048, 40), (33, 64, 65), (64, 128, 64), (64, 1500, 33),
           (65, 136, 72), (130, 200, 20), (129, 96, 257), (300, 64, 512), (515, 72, 136), (1000, 20, 24), (257, 1030, 264), (64, 2056, 128), (2000, 40, 56)]
 
 
@@ -294,8 +294,11 @@ def test_refusals():
     q.act = 0
     assert lib.gcpnet_linear_act_backward(q, None, 4096, 12, None, None, 4096, None, None) == -1  # (db without workspace)
     assert lib.gcpnet_linear_act_workspace(q, 0) == 0 and lib.gcpnet_linear_act_forward(q, None, 0, 4096, None, 8, None) == -1  # (off 16 bytes)
-    q.x = 4098  # (its copy: 4 rows of 8 floats; in a backward dz and the column sums of 256 groups too)
-    assert lib.gcpnet_linear_act_workspace(q, 0) == 32 and lib.gcpnet_linear_act_workspace(q, 1) == 32 + 48 + 256 * 12
+    q.x = 4098  # (off 16 bytes, a copy of 4 rows of 8 floats; in a backward dz and the column sums of 256 groups too)
+    assert lib.gcpnet_linear_act_workspace(q, 0) == 0 and lib.gcpnet_linear_act_workspace(q, 1) == 32 + 48 + 256 * 12
+    q.rows = 65  # (a few rows need no copies)
+    assert lib.gcpnet_linear_act_workspace(q, 0) == 65 * 8
+    q.rows = 4
     q.type = 7
     assert lib.gcpnet_linear_act_workspace(q, 0) == -1
     q.type = 0
