@@ -15,7 +15,6 @@
 namespace {
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 
 constexpr int CHUNK = 4096, QBLOCK = 256, ITER = CHUNK / (4 * QBLOCK);  // four waves x ITER blocks of 256
@@ -24,7 +23,7 @@ constexpr int NORM_CHUNK = 16384;
 struct StepArgs {
     gcp_adamw_tensor_t t[GCP_ADAMW_MAX_TENSORS];
     int first[GCP_ADAMW_MAX_TENSORS + 1];  // first chunk of each tensor
-    const float* corr;                     // {lr / (1 - b1^t), sqrt(1 - b2^t)} of each tensor
+    const float* corr;                     // {lr / (1 - b1^t), 1 / sqrt(1 - b2^t)} of each tensor
     const float* clip;                     // {norm, coefficient} or NULL
     int n;
     float b1, c1, b2, c2, eps, keep;       // c = 1 - b, keep = 1 - lr wd
@@ -40,11 +39,11 @@ __device__ __forceinline__ unsigned mix32(unsigned h) {
     return h ^ (h >> 16);
 }
 
-__device__ __forceinline__ float bf16_to_f(unsigned b) { return __uint_as_float(b << 16); }
-__device__ __forceinline__ unsigned f_to_bf16(float x) {  // nearest even; NaN stays NaN
-    const unsigned u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+// two values as bf16, nearest even (NaN stays NaN), the first in the low half
+__device__ __forceinline__ unsigned bf16_pair(float a, float b) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    const pair p = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(unsigned, p);
 }
 
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }
@@ -68,10 +67,21 @@ __device__ __forceinline__ float e4m3_stochastic(float y, unsigned r) {
     return y >= 0x1p-6f ? whole : small;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
+// The largest of the wave's values, in scalar registers: within rows of 16 lanes, then from row to row.
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+#define STEP(ctrl, rows) { const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false); x = y > x ? y : x; }
+    STEP(0x111, 0xf) STEP(0x112, 0xf) STEP(0x114, 0xf) STEP(0x118, 0xf)  // from 1, 2, 4, 8 lanes below
+    STEP(0x142, 0xa) STEP(0x143, 0xc)                                    // row 0 to 1 and 2 to 3; rows 0 - 1 to 2 - 3
+#undef STEP
+    return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// sqrt and quotient of the parameter's update by the hardware's root and reciprocal, each good to a unit in the last place (the root takes
+// no subnormal numbers: those are scaled).  With the full-precision forms an 8-bit step is bound by arithmetic, not by memory.
+__device__ __forceinline__ float quick_sqrt(float v) {
+    const bool low = v < 0x1p-96f;
+    const float r = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v);
+    return low ? r * 0x1p-32f : r;
 }
 
 // four values of a wave's piece: whole vectors where the tensor's addresses allow them, else element by element, absent ones 0
@@ -85,19 +95,15 @@ __device__ __forceinline__ f32x4 load_f32(const float* p, int64_t i, int64_t n) 
     return x;
 }
 template <bool VEC>
-__device__ __forceinline__ f32x4 load_bf16(const unsigned short* p, int64_t i, int64_t n) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (VEC) {
-        const u32x2 u = *(const u32x2*)(p + i);
-        x[0] = __uint_as_float(u[0] << 16); x[1] = __uint_as_float(u[0] & 0xffff0000u);
-        x[2] = __uint_as_float(u[1] << 16); x[3] = __uint_as_float(u[1] & 0xffff0000u);
-    } else {
+__device__ __forceinline__ u32x2 load_u16x4(const unsigned short* p, int64_t i, int64_t n) {
+    if constexpr (VEC) return *(const u32x2*)(p + i);
+    u32x2 x = {0u, 0u};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j < n) x[j] = bf16_to_f(p[i + j]);
-    }
+    for (int j = 0; j < 4; ++j)
+        if (i + j < n) x[j / 2] |= (unsigned)p[i + j] << (16 * (j & 1));
     return x;
 }
+__device__ __forceinline__ float bf16_of(u32x2 x, int j) { return __uint_as_float(j & 1 ? x[j / 2] & 0xffff0000u : x[j / 2] << 16); }
 template <bool VEC>
 __device__ __forceinline__ unsigned load_u8x4(const unsigned char* p, int64_t i, int64_t n) {
     if constexpr (VEC) return *(const unsigned*)(p + i);
@@ -115,17 +121,11 @@ __device__ __forceinline__ void store_f32(float* p, int64_t i, int64_t n, f32x4 
         if (i + j < n) p[i + j] = x[j];
 }
 template <bool VEC>
-__device__ __forceinline__ void store_bf16(unsigned short* p, int64_t i, int64_t n, f32x4 x) {
-    if constexpr (VEC) {
-        u32x2 u;
-        u[0] = f_to_bf16(x[0]) | f_to_bf16(x[1]) << 16;
-        u[1] = f_to_bf16(x[2]) | f_to_bf16(x[3]) << 16;
-        *(u32x2*)(p + i) = u;
-        return;
-    }
+__device__ __forceinline__ void store_u16x4(unsigned short* p, int64_t i, int64_t n, u32x2 x) {
+    if constexpr (VEC) { *(u32x2*)(p + i) = x; return; }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (i + j < n) p[i + j] = (unsigned short)f_to_bf16(x[j]);
+        if (i + j < n) p[i + j] = (unsigned short)(x[j / 2] >> (16 * (j & 1)));
 }
 template <bool VEC>
 __device__ __forceinline__ void store_u8x4(unsigned char* p, int64_t i, int64_t n, unsigned u) {
@@ -152,7 +152,8 @@ __device__ __forceinline__ unsigned nan_codes(unsigned codes, f32x4 x) {
 }
 
 struct Piece {  // one wave's 256 elements as loaded, four per lane
-    f32x4 p, g, m, v, w;
+    f32x4 p, g, m, v;  // (p: the master copy of a bf16 parameter)
+    u32x2 hp, hg;      // a bf16 parameter and its gradient
     unsigned mc, vc;
     float ms, vs;
 };
@@ -160,9 +161,9 @@ struct Piece {  // one wave's 256 elements as loaded, four per lane
 template <bool BF16, bool EIGHT, bool VEC>
 __device__ __forceinline__ void piece_load(const gcp_adamw_tensor_t& T, int64_t i, Piece& q) {
     if constexpr (BF16) {
-        q.p = load_bf16<VEC>((const unsigned short*)T.param, i, T.n);
-        q.g = load_bf16<VEC>((const unsigned short*)T.grad, i, T.n);
-        q.w = load_f32<VEC>(T.master, i, T.n);
+        q.hp = load_u16x4<VEC>((const unsigned short*)T.param, i, T.n);
+        q.hg = load_u16x4<VEC>((const unsigned short*)T.grad, i, T.n);
+        q.p = load_f32<VEC>(T.master, i, T.n);
     } else {
         q.p = load_f32<VEC>((const float*)T.param, i, T.n);
         q.g = load_f32<VEC>((const float*)T.grad, i, T.n);
@@ -188,43 +189,76 @@ __device__ __forceinline__ void piece_update(const StepArgs& a, const gcp_adamw_
         q.v = e4m3_decode(q.vc);
     }
     f32x4 p = q.p;
+    if constexpr (BF16) {
+        // a parameter that is not the rounding of its master copy was written by somebody else: it is taken as it is
+        const u32x2 diff = {bf16_pair(p[0], p[1]) ^ q.hp[0], bf16_pair(p[2], p[3]) ^ q.hp[1]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((j & 1 ? diff[j / 2] >> 16 : diff[j / 2] & 0xffffu) != 0) p[j] = bf16_of(q.hp, j);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float g = q.g[j] * clip;
+        const float g = (BF16 ? bf16_of(q.hg, j) : q.g[j]) * clip;
         if constexpr (EIGHT) {
             q.m[j] *= q.ms;
             q.v[j] *= q.vs;
         }
-        // a parameter that is not the rounding of its master copy was written by somebody else: it is taken as it is
-        if constexpr (BF16) p[j] = f_to_bf16(q.w[j]) == __float_as_uint(q.p[j]) >> 16 ? q.w[j] : q.p[j];
         q.m[j] = q.m[j] * a.b1 + g * a.c1;
         q.v[j] = q.v[j] * a.b2 + (g * a.c2) * g;
-        p[j] = p[j] * a.keep - lr1 * (q.m[j] / (sqrtf(q.v[j]) / root2 + a.eps));
+        p[j] = p[j] * a.keep - lr1 * (q.m[j] * __builtin_amdgcn_rcpf(quick_sqrt(q.v[j]) * root2 + a.eps));
     }
     if constexpr (BF16) {
-        store_bf16<VEC>((unsigned short*)T.param, i, T.n, p);
+        store_u16x4<VEC>((unsigned short*)T.param, i, T.n, u32x2{bf16_pair(p[0], p[1]), bf16_pair(p[2], p[3])});
         store_f32<VEC>(T.master, i, T.n, p);
     } else {
         store_f32<VEC>((float*)T.param, i, T.n, p);
     }
     if constexpr (EIGHT) {
-        float tm = 0.f, tv = 0.f;
+        unsigned tm = 0, tv = 0;  // (magnitudes as whole numbers, which order like them; absent elements are 0)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {  // (absent elements are 0)
-            if (finite_f(q.m[j])) tm = fmaxf(tm, fabsf(q.m[j]));
-            if (finite_f(q.v[j])) tv = fmaxf(tv, q.v[j]);
+        for (int j = 0; j < 4; ++j) {
+            const unsigned um = __float_as_uint(q.m[j]) & 0x7fffffffu, uv = __float_as_uint(q.v[j]) & 0x7fffffffu;
+            tm = um > tm ? um : tm;
+            tv = uv > tv ? uv : tv;
         }
-        const float ms = block_scale(wave_max(tm)), vs = block_scale(wave_max(tv));
+        tm = wave_max(tm);
+        tv = wave_max(tv);
+        const bool all_finite = tm < 0x7f800000u && tv < 0x7f800000u;
+        if (!all_finite) {  // infinities and NaN get the code of NaN and do not count for the scale
+            unsigned fm = 0, fv = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned um = __float_as_uint(q.m[j]) & 0x7fffffffu, uv = __float_as_uint(q.v[j]) & 0x7fffffffu;
+                if (um < 0x7f800000u && um > fm) fm = um;
+                if (uv < 0x7f800000u && uv > fv) fv = uv;
+            }
+            tm = wave_max(fm);
+            tv = wave_max(fv);
+        }
+        const float ms = block_scale(__uint_as_float(tm)), vs = block_scale(__uint_as_float(tv));
         const float mi = pow2_inverse(ms), vi = pow2_inverse(vs);
         f32x4 ym, yv;
         const unsigned k = i >> 32 ? mix32(key ^ mix32((unsigned)(i >> 32))) : key;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            ym[j] = finite_f(q.m[j]) ? q.m[j] * mi : 0.f;
-            yv[j] = finite_f(q.v[j]) ? e4m3_stochastic(q.v[j] * vi, mix32(k + (unsigned)i + j) & 0xfffffu) : 0.f;
+            ym[j] = q.m[j] * mi;
+            yv[j] = e4m3_stochastic(q.v[j] * vi, mix32(k + (unsigned)i + j) & 0xfffffu);
         }
-        store_u8x4<VEC>((unsigned char*)T.exp_avg, i, T.n, nan_codes(e4m3_encode(ym), q.m));
-        store_u8x4<VEC>((unsigned char*)T.exp_avg_sq, i, T.n, nan_codes(e4m3_encode(yv), q.v));
+        unsigned cm, cv;
+        if (all_finite) {
+            cm = e4m3_encode(ym);
+            cv = e4m3_encode(yv);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!finite_f(q.m[j])) ym[j] = 0.f;
+                if (!finite_f(q.v[j])) yv[j] = 0.f;
+            }
+            cm = nan_codes(e4m3_encode(ym), q.m);
+            cv = nan_codes(e4m3_encode(yv), q.v);
+        }
+        store_u8x4<VEC>((unsigned char*)T.exp_avg, i, T.n, cm);
+        store_u8x4<VEC>((unsigned char*)T.exp_avg_sq, i, T.n, cv);
         if ((threadIdx.x & 63) == 0) {
             T.exp_avg_scale[i / QBLOCK] = ms;
             T.exp_avg_sq_scale[i / QBLOCK] = vs;
@@ -248,21 +282,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs a) {
     const float clip = a.clip ? a.clip[1] : 1.f, lr1 = a.corr[2 * lo], root2 = a.corr[2 * lo + 1];
     unsigned key = 0;
     if constexpr (EIGHT) key = mix32(mix32(a.seed + 0x9e3779b9u * T.ordinal) ^ (unsigned)(int)*T.step);
-    if (T.vec && at + CHUNK <= T.n) {
-        Piece q[ITER];
+    Piece q[ITER];
 #pragma unroll
-        for (int k = 0; k < ITER; ++k) piece_load<BF16, EIGHT, true>(T, at + (k * 4 + wave) * QBLOCK + 4 * lane, q[k]);
+    for (int k = 0; k < ITER; ++k) {  // (uniform over a wave: a whole piece, the end of the tensor, or nothing)
+        const int64_t b = at + (k * 4 + wave) * QBLOCK;
+        if (T.vec && b + QBLOCK <= T.n) piece_load<BF16, EIGHT, true>(T, b + 4 * lane, q[k]);
+        else if (b < T.n) piece_load<BF16, EIGHT, false>(T, b + 4 * lane, q[k]);
+    }
 #pragma unroll
-        for (int k = 0; k < ITER; ++k)
-            piece_update<BF16, EIGHT, true>(a, T, at + (k * 4 + wave) * QBLOCK + 4 * lane, q[k], clip, lr1, root2, key);
-    } else {
-        for (int k = 0; k < ITER; ++k) {
-            const int64_t b = at + (k * 4 + wave) * QBLOCK;
-            if (b >= T.n) break;  // (wave-uniform)
-            Piece q;
-            piece_load<BF16, EIGHT, false>(T, b + 4 * lane, q);
-            piece_update<BF16, EIGHT, false>(a, T, b + 4 * lane, q, clip, lr1, root2, key);
-        }
+    for (int k = 0; k < ITER; ++k) {
+        const int64_t b = at + (k * 4 + wave) * QBLOCK;
+        if (T.vec && b + QBLOCK <= T.n) piece_update<BF16, EIGHT, true>(a, T, b + 4 * lane, q[k], clip, lr1, root2, key);
+        else if (b < T.n) piece_update<BF16, EIGHT, false>(a, T, b + 4 * lane, q[k], clip, lr1, root2, key);
     }
 }
 
@@ -285,7 +316,7 @@ __global__ __launch_bounds__(512) void adamw_begin_kernel(BeginArgs a) {
         const float t = *a.step[i] + 1.f;
         *a.step[i] = t;
         a.corr[2 * i] = (float)(a.lr / (1.0 - pow(a.b1, (double)t)));
-        a.corr[2 * i + 1] = (float)sqrt(1.0 - pow(a.b2, (double)t));
+        a.corr[2 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t)));
     }
     if (!a.part) return;
     __shared__ double sums[512];
@@ -322,8 +353,12 @@ __device__ __forceinline__ float square_sum(const void* g, int64_t at, int64_t n
     for (int k = 0; k < NORM_CHUNK / 1024; ++k) {
         const int64_t i = at + k * 1024 + 4 * (int)threadIdx.x;
         f32x4 x;
-        if constexpr (BF16) x = load_bf16<VEC>((const unsigned short*)g, i, n);
-        else x = load_f32<VEC>((const float*)g, i, n);
+        if constexpr (BF16) {
+            const u32x2 h = load_u16x4<VEC>((const unsigned short*)g, i, n);
+            x = f32x4{bf16_of(h, 0), bf16_of(h, 1), bf16_of(h, 2), bf16_of(h, 3)};
+        } else {
+            x = load_f32<VEC>((const float*)g, i, n);
+        }
         s += (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
     }
     return s;

@@ -397,12 +397,13 @@ bool by_shape(int d, F f) {
 #undef TRY
     return false;
 }
-// Workgroups of the backward: as many as the registers let reside on 256 CUs, each walking many rows.
+// Workgroups of the backward: as many as the registers let reside on 256 CUs, each walking many rows, but four turns before there are more of
+// them than CUs (the partial sums of each have to be added).
 template <class E, int G, int NV>
 int64_t backward_blocks(int64_t rows) {
     constexpr int T = G > 256 ? G : 256, most = T > 256 ? 256 : NV > 1 ? 512 : E::vec == 8 ? 768 : 1024;
-    const int64_t blocks = (rows + T / G - 1) / (T / G);
-    return blocks < most ? blocks : most;
+    const int64_t blocks = (rows + T / G - 1) / (T / G), few = blocks < 256 ? blocks : blocks < 1024 ? 256 : blocks / 4;
+    return few < most ? few : most;
 }
 
 template <class F>

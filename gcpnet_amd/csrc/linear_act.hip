@@ -441,27 +441,37 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
     float sum[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = 0.f;
-    if (count > 0) {
-#pragma unroll 4
-        for (int64_t r = (int64_t)blockIdx.y * TY + ty; r < a.rows; r += (int64_t)gridDim.y * TY) {
-            const Raw<E, V> dy = elem_load<E, V>(a.dy, r * a.dy_ld + c, count);
-            float v[V];
+    const int64_t step = (int64_t)gridDim.y * TY;
+    if (count > 0)
+        for (int64_t r0 = (int64_t)blockIdx.y * TY + ty; r0 < a.rows; r0 += 4 * step) {  // four rows requested at a time
+            Raw<E, V> dy[4], zr[4];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = dy[j];
-            if (a.act != GCP_ACT_NONE) {
-                const Raw<E, V> zr = elem_load<E, V>(a.z, r * a.n + c, count);
-                float z[V], act[V], d[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) z[j] = zr[j];
-                elem_act<V, true>(a.act, a.slope, z, act, d);
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = j < count ? v[j] * d[j] : 0.f;
+            for (int u = 0; u < 4; ++u) {
+                const int64_t r = r0 + u * step;
+                if (r >= a.rows) continue;
+                dy[u] = elem_load<E, V>(a.dy, r * a.dy_ld + c, count);
+                if (a.act != GCP_ACT_NONE) zr[u] = elem_load<E, V>(a.z, r * a.n + c, count);
             }
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] += v[j];
-            if (a.dz) elem_store<E, V>(a.dz, r * a.dz_ld + c, v);  // (whole pieces: dz_ld is a multiple of them)
+            for (int u = 0; u < 4; ++u) {
+                const int64_t r = r0 + u * step;
+                if (r >= a.rows) continue;
+                float v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = dy[u][j];
+                if (a.act != GCP_ACT_NONE) {
+                    float z[V], act[V], d[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) z[j] = zr[u][j];
+                    elem_act<V, true>(a.act, a.slope, z, act, d);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[j] = j < count ? v[j] * d[j] : 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += v[j];
+                if (a.dz) elem_store<E, V>(a.dz, r * a.dz_ld + c, v);  // (whole pieces: dz_ld is a multiple of them)
+            }
         }
-    }
     if (!a.part) return;
 #pragma unroll
     for (int j = 0; j < V; ++j) cols[threadIdx.x * V + j] = sum[j];
@@ -587,7 +597,7 @@ int product(int64_t m, int64_t n, int64_t k, const Mat& a, bool a_across, const 
     return 0;
 }
 
-constexpr int DZ_GROUPS = 256;
+constexpr int DZ_GROUPS = 512;
 
 int check_desc(const gcp_linear_t* l) {
     if (!l || l->rows < 0 || l->k < 1 || l->n < 1 || !elem_type_ok(l->type) || l->act < 0 || l->act > GCP_ACT_SIGMOID) return GCPNET_E_BADARG;
@@ -674,8 +684,8 @@ extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, 
             a.tx = 8;
             while (a.tx < 256 && a.tx < across) a.tx *= 2;
             const int64_t bx = (across + a.tx - 1) / a.tx, ty = 256 / a.tx;
-            // (two workgroups per CU in all; a thread takes eight rows or more before there are more groups of rows)
-            int64_t by = (l->rows + 8 * ty - 1) / (8 * ty), most = (512 + bx - 1) / bx;
+            // (four workgroups per CU in all; a thread takes four rows or more before there are more groups of rows)
+            int64_t by = (l->rows + 4 * ty - 1) / (4 * ty), most = (1024 + bx - 1) / bx;
             by = by < most ? by : most;
             by = by < DZ_GROUPS ? by : DZ_GROUPS;
             if (by > 0) {

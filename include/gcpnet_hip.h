@@ -595,7 +595,7 @@ typedef struct {
 /* floats that gcpnet_grad_norm writes: sums of squares over 16384 elements each */
 int64_t gcpnet_grad_norm_partials(int n, const gcp_adamw_tensor_t* tensors);
 int gcpnet_grad_norm(int n, const gcp_adamw_tensor_t* tensors, int type, float* partials, void* stream);
-/* step += 1 and corrections[2 k], [2 k + 1] = lr / (1 - beta1^step), sqrt(1 - beta2^step) for every tensor; with `partials` also
+/* step += 1 and corrections[2 k], [2 k + 1] = lr / (1 - beta1^step), 1 / sqrt(1 - beta2^step) for every tensor; with `partials` also
  * clip[0], clip[1] = norm, min(1, max_norm / (norm + 1e-6)) */
 int gcpnet_adamw_begin(int n, const gcp_adamw_tensor_t* tensors, double lr, double beta1, double beta2, float* corrections,
                        const float* partials, int64_t n_partials, float max_norm, float* clip, void* stream);

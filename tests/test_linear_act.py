@@ -294,8 +294,8 @@ def test_refusals():
     q.act = 0
     assert lib.gcpnet_linear_act_backward(q, None, 4096, 12, None, None, 4096, None, None) == -1  # (db without workspace)
     assert lib.gcpnet_linear_act_workspace(q, 0) == 0 and lib.gcpnet_linear_act_forward(q, None, 0, 4096, None, 8, None) == -1  # (off 16 bytes)
-    q.x = 4098  # (off 16 bytes, a copy of 4 rows of 8 floats; in a backward dz and the column sums of 256 groups too)
-    assert lib.gcpnet_linear_act_workspace(q, 0) == 0 and lib.gcpnet_linear_act_workspace(q, 1) == 32 + 48 + 256 * 12
+    q.x = 4098  # (off 16 bytes, a copy of 4 rows of 8 floats; in a backward dz and the column sums of 512 groups too)
+    assert lib.gcpnet_linear_act_workspace(q, 0) == 0 and lib.gcpnet_linear_act_workspace(q, 1) == 32 + 48 + 512 * 12
     q.rows = 65  # (a few rows need no copies)
     assert lib.gcpnet_linear_act_workspace(q, 0) == 65 * 8
     q.rows = 4
