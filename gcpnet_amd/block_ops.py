@@ -121,12 +121,21 @@ def _norm_backward(ctx, ds, dh):
         b.gate_ld = g2.stride(0)
     lib = _lib.load()
     new = lambda want, like: s.new_empty(like) if want else None  # noqa: E731
-    dx, dy, dgate = new(need_x, shape), new(need_y and y2 is not None, shape), new(need_gate and g2 is not None, gate_shape)
+    dx, dy = new(need_x, shape), new(need_y and y2 is not None, shape)
+    need_gate = need_gate and g2 is not None
+    dgate = new(need_gate and not ctx.channel, gate_shape)
     dws = [None] * 4
     wanted = [i for i in range(4) if need_w[i] and ws[i] is not None]
-    if wanted:  # (one allocation: they are short)
-        for i, v in zip(wanted, ws[wanted[0]].new_empty((len(wanted), n.d)).unbind()):
-            dws[i] = v
+    dtype = ws[wanted[0]].dtype if wanted else s.dtype
+    together = need_gate and ctx.channel and dtype == s.dtype  # (one allocation for the short ones)
+    if wanted or together:
+        short = iter(s.new_empty((len(wanted) + together, n.d), dtype=dtype).unbind())
+        for i in wanted:
+            dws[i] = next(short)
+        if together:
+            dgate = next(short)
+    if need_gate and dgate is None:
+        dgate = new(True, gate_shape)
     scratch = None
     if wanted or (dgate is not None and ctx.channel):
         scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(C.byref(b)))), dtype=torch.float32, device=s.device)

@@ -10,6 +10,8 @@
 // mixture of sizes fill the chip.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -19,17 +21,29 @@ typedef float f32x2v __attribute__((ext_vector_type(2)));
 
 constexpr int CHUNK = 4096, QBLOCK = 256, ITER = CHUNK / (4 * QBLOCK);  // four waves x ITER blocks of 256
 constexpr int NORM_CHUNK = 16384;
+constexpr int MAX_BEGIN = 448, MAX_NORM = 200;  // tensors per launch of the kernels before the update
 
+// A tensor as the update takes it: no more than its kind needs, so that a launch takes as many as its arguments hold.
+struct Plain { void *param; const void* grad; void *exp_avg, *exp_avg_sq; int64_t n_vec; };  // n_vec: 2 n + (16-byte accesses)
+struct Master { float* master; };
+struct Scales { float *exp_avg_scale, *exp_avg_sq_scale; uint32_t ordinal, unused; };
+struct Nothing1 {};
+struct Nothing2 {};
+template <bool BF16, bool EIGHT>
+struct Slot : Plain, std::conditional_t<BF16, Master, Nothing1>, std::conditional_t<EIGHT, Scales, Nothing2> {};
+
+template <bool BF16, bool EIGHT>
 struct StepArgs {
-    gcp_adamw_tensor_t t[GCP_ADAMW_MAX_TENSORS];
-    int first[GCP_ADAMW_MAX_TENSORS + 1];  // first chunk of each tensor
-    const float* corr;                     // {lr / (1 - b1^t), 1 / sqrt(1 - b2^t)} of each tensor
-    const float* clip;                     // {norm, coefficient} or NULL
+    static constexpr int MOST = (4096 - 64) / (int)(sizeof(Slot<BF16, EIGHT>) + sizeof(int));
+    Slot<BF16, EIGHT> t[MOST];
+    int first[MOST + 1];   // first chunk of each tensor
+    const float* corr;     // {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), t, -} of each tensor
+    const float* clip;     // {norm, coefficient} or NULL
     int n;
-    float b1, c1, b2, c2, eps, keep;       // c = 1 - b, keep = 1 - lr wd
+    float b1, c1, b2, c2, eps, keep;  // c = 1 - b, keep = 1 - lr wd
     unsigned seed;
 };
-static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(StepArgs<false, false>) <= 4096 && sizeof(StepArgs<true, true>) <= 4096, "kernel arguments");
 
 __device__ __forceinline__ unsigned mix32(unsigned h) {
     h ^= h >> 16;
@@ -180,7 +194,7 @@ __device__ __forceinline__ void piece_load(const gcp_adamw_tensor_t& T, int64_t 
 }
 
 template <bool BF16, bool EIGHT, bool VEC>
-__device__ __forceinline__ void piece_update(const StepArgs& a, const gcp_adamw_tensor_t& T, int64_t i, Piece& q, float clip, float lr1,
+__device__ __forceinline__ void piece_update(const StepArgs<BF16, EIGHT>& a, const gcp_adamw_tensor_t& T, int64_t i, Piece& q, float clip, float lr1,
                                              float root2, unsigned key) {
     // (products and sums of the moments rounded one by one: the codes of 8-bit moments are then the same wherever they are computed)
 #pragma clang fp contract(off)
@@ -270,18 +284,24 @@ __device__ __forceinline__ void piece_update(const StepArgs& a, const gcp_adamw_
 }
 
 template <bool BF16, bool EIGHT>
-__global__ __launch_bounds__(256) void adamw_kernel(StepArgs a) {
+__global__ __launch_bounds__(256) void adamw_kernel(StepArgs<BF16, EIGHT> a) {
     int lo = 0, hi = a.n - 1;  // the tensor of this chunk
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (a.first[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
     }
-    const gcp_adamw_tensor_t& T = a.t[lo];
+    const Slot<BF16, EIGHT>& slot = a.t[lo];
+    gcp_adamw_tensor_t T;
+    T.param = slot.param; T.grad = slot.grad; T.exp_avg = slot.exp_avg; T.exp_avg_sq = slot.exp_avg_sq;
+    T.n = slot.n_vec >> 1;
+    T.vec = (int)(slot.n_vec & 1);
+    if constexpr (BF16) T.master = slot.master;
+    if constexpr (EIGHT) { T.exp_avg_scale = slot.exp_avg_scale; T.exp_avg_sq_scale = slot.exp_avg_sq_scale; }
     const int64_t at = (int64_t)((int)blockIdx.x - a.first[lo]) * CHUNK;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float clip = a.clip ? a.clip[1] : 1.f, lr1 = a.corr[2 * lo], root2 = a.corr[2 * lo + 1];
+    const float clip = a.clip ? a.clip[1] : 1.f, lr1 = a.corr[4 * lo], root2 = a.corr[4 * lo + 1];
     unsigned key = 0;
-    if constexpr (EIGHT) key = mix32(mix32(a.seed + 0x9e3779b9u * T.ordinal) ^ (unsigned)(int)*T.step);
+    if constexpr (EIGHT) key = mix32(mix32(a.seed + 0x9e3779b9u * slot.ordinal) ^ (unsigned)(int)a.corr[4 * lo + 2]);
     Piece q[ITER];
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {  // (uniform over a wave: a whole piece, the end of the tensor, or nothing)
@@ -297,10 +317,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs a) {
     }
 }
 
-// Before the update: the step counts of up to GCP_ADAMW_MAX_BEGIN tensors advance in device memory (so that a captured step counts on),
+// Before the update: the step counts of up to MAX_BEGIN tensors advance in device memory (so that a captured step counts on),
 // their bias corrections are formed in double, and the partial sums of the squared gradients become the norm and the coefficient.
 struct BeginArgs {
-    float* step[GCP_ADAMW_MAX_BEGIN];
+    float* step[MAX_BEGIN];
     int n;
     float* corr;
     double lr, b1, b2;
@@ -315,8 +335,9 @@ __global__ __launch_bounds__(512) void adamw_begin_kernel(BeginArgs a) {
     for (int i = threadIdx.x; i < a.n; i += 512) {
         const float t = *a.step[i] + 1.f;
         *a.step[i] = t;
-        a.corr[2 * i] = (float)(a.lr / (1.0 - pow(a.b1, (double)t)));
-        a.corr[2 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t)));
+        a.corr[4 * i] = (float)(a.lr / (1.0 - pow(a.b1, (double)t)));
+        a.corr[4 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t)));
+        a.corr[4 * i + 2] = t;
     }
     if (!a.part) return;
     __shared__ double sums[512];
@@ -338,9 +359,9 @@ __global__ __launch_bounds__(512) void adamw_begin_kernel(BeginArgs a) {
 
 // One partial sum of squares for every 16384 elements, in an order that does not depend on the launch.
 struct NormArgs {
-    const void* grad[GCP_ADAMW_MAX_NORM];
-    int64_t n[GCP_ADAMW_MAX_NORM];
-    int first[GCP_ADAMW_MAX_NORM + 1];
+    const void* grad[MAX_NORM];
+    int64_t n[MAX_NORM];
+    int first[MAX_NORM + 1];
     int count, bf16;
     float* part;
 };
@@ -384,6 +405,44 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(NormArgs a) {
 
 bool aligned(const void* p, unsigned b) { return ((uintptr_t)p & (b - 1)) == 0; }
 
+struct Options { double lr, beta1, beta2, eps, weight_decay; uint32_t seed; };
+
+template <bool BF16, bool EIGHT>
+int launch_steps(int n, const gcp_adamw_tensor_t* t, const Options& o, const float* corrections, const float* clip, hipStream_t stream) {
+    for (int k = 0; k < n;) {
+        StepArgs<BF16, EIGHT> a;
+        a.n = 0;
+        const int k0 = k;
+        int64_t c = 0;
+        for (; k < n && a.n < a.MOST; ++k) {
+            const int64_t more = (t[k].n + CHUNK - 1) / CHUNK;
+            if (more > INT32_MAX / 2) return GCPNET_E_UNSUPPORTED;
+            if (c + more > INT32_MAX / 2) break;
+            Slot<BF16, EIGHT>& s = a.t[a.n];
+            s.param = t[k].param; s.grad = t[k].grad; s.exp_avg = t[k].exp_avg; s.exp_avg_sq = t[k].exp_avg_sq;
+            const unsigned w = BF16 ? 8 : 16, q = EIGHT ? 4 : 16;
+            const bool vec = aligned(t[k].param, w) && aligned(t[k].grad, w) && aligned(t[k].exp_avg, q) && aligned(t[k].exp_avg_sq, q) &&
+                             (!BF16 || aligned(t[k].master, 16));
+            s.n_vec = 2 * t[k].n + (vec ? 1 : 0);
+            if constexpr (BF16) s.master = t[k].master;
+            if constexpr (EIGHT) { s.exp_avg_scale = t[k].exp_avg_scale; s.exp_avg_sq_scale = t[k].exp_avg_sq_scale; s.ordinal = t[k].ordinal; s.unused = 0; }
+            a.first[a.n++] = (int)c;
+            c += more;
+        }
+        a.first[a.n] = (int)c;
+        if (!c) continue;
+        a.corr = corrections + 4 * (int64_t)k0;
+        a.clip = clip;
+        a.b1 = (float)o.beta1; a.c1 = (float)(1.0 - o.beta1);
+        a.b2 = (float)o.beta2; a.c2 = (float)(1.0 - o.beta2);
+        a.eps = (float)o.eps; a.keep = (float)(1.0 - o.lr * o.weight_decay);
+        a.seed = o.seed;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw_kernel<BF16, EIGHT>), dim3((unsigned)c), dim3(256), 0, stream, a);
+        GCP_HIP_CHECK_LAUNCH();
+    }
+    return 0;
+}
+
 }  // namespace
 
 extern "C" int64_t gcpnet_grad_norm_partials(int n, const gcp_adamw_tensor_t* t) {
@@ -404,7 +463,7 @@ extern "C" int gcpnet_grad_norm(int n, const gcp_adamw_tensor_t* t, int type, fl
         NormArgs a;
         int64_t c = 0;
         a.count = 0;
-        for (; k < n && a.count < GCP_ADAMW_MAX_NORM; ++k) {
+        for (; k < n && a.count < MAX_NORM; ++k) {
             if (t[k].n == 0) continue;
             const int64_t more = (t[k].n + NORM_CHUNK - 1) / NORM_CHUNK;
             if (more > INT32_MAX / 2) return GCPNET_E_UNSUPPORTED;
@@ -429,11 +488,11 @@ extern "C" int gcpnet_adamw_begin(int n, const gcp_adamw_tensor_t* t, double lr,
     if (n < 0 || (n > 0 && (!t || !corrections)) || (partials && !clip) || n_partials < 0) return GCPNET_E_BADARG;
     for (int k = 0; k < n; ++k)
         if (!t[k].step) return GCPNET_E_BADARG;
-    for (int k = 0; k < n || (k == 0 && partials); k += GCP_ADAMW_MAX_BEGIN) {
+    for (int k = 0; k < n || (k == 0 && partials); k += MAX_BEGIN) {
         BeginArgs a = {};
-        a.n = n - k < GCP_ADAMW_MAX_BEGIN ? n - k : GCP_ADAMW_MAX_BEGIN;
+        a.n = n - k < MAX_BEGIN ? n - k : MAX_BEGIN;
         for (int j = 0; j < a.n; ++j) a.step[j] = t[k + j].step;
-        a.corr = corrections + 2 * (int64_t)k;
+        a.corr = corrections + 4 * (int64_t)k;
         a.lr = lr; a.b1 = beta1; a.b2 = beta2;
         a.part = k == 0 ? partials : nullptr;
         a.n_part = n_partials; a.max_norm = max_norm; a.clip = clip;
@@ -454,35 +513,7 @@ extern "C" int gcpnet_adamw_step(int n, const gcp_adamw_tensor_t* t, int type, i
                            (eight && (!t[k].exp_avg_scale || !t[k].exp_avg_sq_scale))))
             return GCPNET_E_BADARG;
     }
-    for (int k = 0; k < n;) {
-        StepArgs a;
-        a.n = 0;
-        const int k0 = k;
-        int64_t c = 0;
-        for (; k < n && a.n < GCP_ADAMW_MAX_TENSORS; ++k) {
-            const int64_t more = (t[k].n + CHUNK - 1) / CHUNK;
-            if (more > INT32_MAX / 2) return GCPNET_E_UNSUPPORTED;
-            if (c + more > INT32_MAX / 2) break;
-            a.t[a.n] = t[k];
-            const unsigned w = half ? 8 : 16, s = eight ? 4 : 16;
-            a.t[a.n].vec = aligned(t[k].param, w) && aligned(t[k].grad, w) && aligned(t[k].exp_avg, s) && aligned(t[k].exp_avg_sq, s) &&
-                           (!half || aligned(t[k].master, 16));
-            a.first[a.n++] = (int)c;
-            c += more;
-        }
-        a.first[a.n] = (int)c;
-        if (!c) continue;
-        a.corr = corrections + 2 * (int64_t)k0;
-        a.clip = clip;
-        a.b1 = (float)beta1; a.c1 = (float)(1.0 - beta1);
-        a.b2 = (float)beta2; a.c2 = (float)(1.0 - beta2);
-        a.eps = (float)eps; a.keep = (float)(1.0 - lr * weight_decay);
-        a.seed = seed;
-#define ADAMW_LAUNCH(B, E) hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw_kernel<B, E>), dim3((unsigned)c), dim3(256), 0, (hipStream_t)stream, a)
-        if (half) { if (eight) ADAMW_LAUNCH(true, true); else ADAMW_LAUNCH(true, false); }
-        else { if (eight) ADAMW_LAUNCH(false, true); else ADAMW_LAUNCH(false, false); }
-#undef ADAMW_LAUNCH
-        GCP_HIP_CHECK_LAUNCH();
-    }
-    return 0;
+    const Options o = {lr, beta1, beta2, eps, weight_decay, seed};
+    if (half) return eight ? launch_steps<true, true>(n, t, o, corrections, clip, (hipStream_t)stream) : launch_steps<true, false>(n, t, o, corrections, clip, (hipStream_t)stream);
+    return eight ? launch_steps<false, true>(n, t, o, corrections, clip, (hipStream_t)stream) : launch_steps<false, false>(n, t, o, corrections, clip, (hipStream_t)stream);
 }

@@ -180,20 +180,23 @@ __device__ __forceinline__ void wait_loads_and_meet() {  // this wave's direct l
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+template <int BM, int BN, int RING>
+constexpr int ring_bytes() { return RING * (BM + BN) * KROW; }
+
+// One tile of C: tile number `block` of the product, piece `piece` of k.
 template <class E, bool AC, bool BC, int BM, int BN, int WM, int WN, int RING>
-__global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
+__device__ __forceinline__ void gemm_tile(const Gemm& g, int block, int piece, char* lds) {
     constexpr int THREADS = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
     typedef Tile<E, AC, BM, THREADS> TA;
     typedef Tile<E, BC, BN, THREADS> TB;
     constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::TURNS + TB::TURNS;
-    __shared__ __attribute__((aligned(16))) char lds[RING * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
 
     const int total = g.tiles_m * g.tiles_n;
     int tm, tn;
-    gcp_tile_of_block((int)blockIdx.x, total, g.tiles_m, g.tiles_n, tm, tn);
+    gcp_tile_of_block(block, total, g.tiles_m, g.tiles_n, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    const int64_t k0 = (int64_t)blockIdx.y * g.k_per, k1 = k0 + g.k_per < g.k ? k0 + g.k_per : g.k;
+    const int64_t k0 = (int64_t)piece * g.k_per, k1 = k0 + g.k_per < g.k ? k0 + g.k_per : g.k;
     const int steps = k1 > k0 ? (int)((k1 - k0 + TA::KE - 1) / TA::KE) : 0;
     const int whole = steps > 0 ? (int)((k1 - k0) / TA::KE) : 0;  // tiles that do not reach past the end of k
 
@@ -312,13 +315,32 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
 #pragma unroll
                     for (int h = 0; h < V; h += 4) {
                         const float four[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
-                        elem_store<ElemF32, 4>(g.part, ((int64_t)blockIdx.y * g.m + m) * g.n + n + h, four, count - h < 4 ? count - h : 4);
+                        elem_store<ElemF32, 4>(g.part, ((int64_t)piece * g.m + m) * g.n + n + h, four, count - h < 4 ? count - h : 4);
                     }
                 } else {
                     finish<E, V>(g.e, m, n, g.n, count, bias, res[u], v);
                 }
             }
         }
+    }
+}
+
+template <class E, bool AC, bool BC, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM * WN * 64, 2) void gemm_kernel(Gemm g) {
+    __shared__ __attribute__((aligned(16))) char lds[ring_bytes<BM, BN, RING>()];
+    gemm_tile<E, AC, BC, BM, BN, WM, WN, RING>(g, (int)blockIdx.x, (int)blockIdx.y, lds);
+}
+
+// Both products of a backward in one launch: dx = dz W in the first workgroups, dW = dz^T x in the others, so that small ones run side by side.
+template <class E, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM * WN * 64, 2) void gemm_pair_kernel(Gemm dx, Gemm dw) {
+    __shared__ __attribute__((aligned(16))) char lds[ring_bytes<BM, BN, RING>()];
+    const int tiles = dx.tiles_m * dx.tiles_n, first = tiles * dx.splits, block = (int)blockIdx.x;
+    if (block < first) {
+        gemm_tile<E, false, true, BM, BN, WM, WN, RING>(dx, block % tiles, block / tiles, lds);
+    } else {
+        const int other = dw.tiles_m * dw.tiles_n;
+        gemm_tile<E, true, true, BM, BN, WM, WN, RING>(dw, (block - first) % other, (block - first) / other, lds);
     }
 }
 
@@ -555,46 +577,64 @@ int put_in_pieces(Mat* const* mats, int n, float*& space, hipStream_t stream) {
     return 0;
 }
 
-template <class E, bool AC, bool BC>
-int launch_tiles(const Gemm& g, int shape, hipStream_t stream) {
-    const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits);
-    const int64_t groups = (int64_t)grid.x * grid.y;
-    // A longer ring hides more of the memory's latency, a shorter one lets more workgroups reside: few of them take the longer (2048^3 bf16, 256
-    // tiles of 128: 23.3 us with three, 26.4 with two; 500 x 4096 x 4096, 512 tiles of 64: 30.7 us with four, 36.0 with two; 3000 x 500 x 2001,
-    // 384 tiles of 128: 25.9 us with three, 22.9 with two; 2048^3 in 1024 tiles of 64: 35.0 with four, 27.2 with two).
-    if (shape == 0 && groups <= 512) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2, 4>), grid, dim3(256), 0, stream, g);
-    else if (shape == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 64, 64, 2, 2, 2>), grid, dim3(256), 0, stream, g);
-    else if (shape == 1 && groups <= 256) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 4, 3>), grid, dim3(512), 0, stream, g);
-    else if (shape == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 128, 128, 2, 4, 2>), grid, dim3(512), 0, stream, g);
-    else if constexpr (E::code != GCP_TYPE_F32) hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, 256, 256, 2, 4, 2>), grid, dim3(512), 0, stream, g);
-    GCP_HIP_CHECK_LAUNCH();
-    return 0;
+// A longer ring hides more of the memory's latency, a shorter one lets more workgroups reside: few of them take the longer (2048^3 bf16, 256
+// tiles of 128: 23.3 us with three, 26.4 with two; 500 x 4096 x 4096, 512 tiles of 64: 30.7 us with four, 36.0 with two; 3000 x 500 x 2001,
+// 384 tiles of 128: 25.9 us with three, 22.9 with two; 2048^3 in 1024 tiles of 64: 35.0 with four, 27.2 with two).
+int form_of(int shape, int64_t groups) { return shape == 0 ? (groups <= 512 ? 0 : 1) : shape == 1 ? (groups <= 256 ? 2 : 3) : 4; }
+
+template <class F>
+void by_form(int form, F f) {
+#define FORM(bm, wn, ring) f(std::integral_constant<int, bm>(), std::integral_constant<int, wn>(), std::integral_constant<int, ring>())
+    switch (form) {
+        case 0: FORM(64, 2, 4); break;
+        case 1: FORM(64, 2, 2); break;
+        case 2: FORM(128, 4, 3); break;
+        case 3: FORM(128, 4, 2); break;
+        default: FORM(256, 4, 2);
+    }
+#undef FORM
 }
 
 // C[m][n] = sum_k A[m][k] B[n][k] with the epilogue; A and B in pieces, as [m][k] and [n][k] or, across, [k][m] and [k][n].
-// ws: gcp_linear_plan(m, n, k, size).floats of workspace.
 template <class E>
-int product(int64_t m, int64_t n, int64_t k, const Mat& a, bool a_across, const Mat& b, bool b_across, const Epilogue& e, float* ws, hipStream_t stream) {
+int describe(Gemm& g, int& shape, int64_t m, int64_t n, int64_t k, const Mat& a, bool a_across, const Mat& b, bool b_across, const Epilogue& e, float*& ws) {
     const GcpLinearPlan plan = gcp_linear_plan(m, n, k, (int)sizeof(typename E::type));
-    if (plan.tiles_m > INT32_MAX / plan.tiles_n) return GCPNET_E_UNSUPPORTED;
+    if (plan.tiles_m * plan.splits > INT32_MAX / 2 / plan.tiles_n) return GCPNET_E_UNSUPPORTED;
     if (plan.splits > 1 && !ws) return GCPNET_E_BADARG;
-    Gemm g = {};
+    shape = plan.shape;
+    g = {};
     g.m = m; g.n = n; g.k = k;
     g.a = a.p; g.a_ld = a.ld; g.b = b.p; g.b_ld = b.ld;
     g.a_rows = a_across ? a.wide : m;
     g.b_rows = b_across ? b.wide : n;
     g.tiles_m = (int)plan.tiles_m; g.tiles_n = (int)plan.tiles_n; g.splits = plan.splits; g.k_per = plan.k_per;
-    g.part = plan.splits > 1 ? ws : nullptr;
+    if (plan.splits > 1) {
+        g.part = ws;
+        ws += (plan.floats + 3) / 4 * 4;
+    }
     g.e = e;
-    int rc;
-    if (!a_across && !b_across) rc = launch_tiles<E, false, false>(g, plan.shape, stream);
-    else if (!a_across) rc = launch_tiles<E, false, true>(g, plan.shape, stream);
-    else rc = launch_tiles<E, true, true>(g, plan.shape, stream);
-    if (rc || plan.splits == 1) return rc;
-    const int64_t vecs = m * ((n + E::vec - 1) / E::vec), blocks = (vecs + 255) / 256;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(join_kernel<E>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, g.part, plan.splits, m, n, e);
+    return 0;
+}
+
+template <class E>
+int join(const Gemm& g, hipStream_t stream) {
+    if (g.splits == 1) return 0;
+    const int64_t vecs = g.m * ((g.n + E::vec - 1) / E::vec), blocks = (vecs + 255) / 256;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(join_kernel<E>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, g.part, g.splits, g.m, g.n, g.e);
     GCP_HIP_CHECK_LAUNCH();
     return 0;
+}
+
+template <class E, bool AC, bool BC>
+int launch(const Gemm& g, int shape, hipStream_t stream) {
+    const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits);
+    by_form(form_of(shape, (int64_t)grid.x * grid.y), [&](auto b, auto wn, auto ring) {
+        constexpr int B = b.value, WN = wn.value;
+        if constexpr (B < 256 || E::code != GCP_TYPE_F32)
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_kernel<E, AC, BC, B, B, 2, WN, ring.value>), grid, dim3(128 * WN), 0, stream, g);
+    });
+    GCP_HIP_CHECK_LAUNCH();
+    return join<E>(g, stream);
 }
 
 constexpr int DZ_GROUPS = 512;
@@ -620,9 +660,9 @@ extern "C" int64_t gcpnet_linear_act_workspace(const gcp_linear_t* l, int backwa
     if (!backward && rows <= GCP_FEW_ROWS) return 0;
     if (rows > 0 && !in_pieces(l->x, l->x_ld, l->k, size)) copies += copy_floats(rows, l->k, size);
     if (rows > 0 && !in_pieces(l->w, l->w_ld, l->k, size)) copies += copy_floats(l->n, l->k, size);
-    if (!backward) return copies + gcp_linear_plan(rows, l->n, l->k, size).floats;
+    if (!backward) return copies + (gcp_linear_plan(rows, l->n, l->k, size).floats + 3) / 4 * 4;
     copies += copy_floats(rows, l->n, size);  // dz, or a copy of dy
-    const int64_t parts = larger(gcp_linear_plan(rows, l->k, l->n, size).floats, gcp_linear_plan(l->n, l->k, rows, size).floats);
+    const int64_t parts = (gcp_linear_plan(rows, l->k, l->n, size).floats + 3) / 4 * 4 + (gcp_linear_plan(l->n, l->k, rows, size).floats + 3) / 4 * 4;
     return copies + larger(parts, (int64_t)DZ_GROUPS * l->n);
 }
 
@@ -648,7 +688,10 @@ extern "C" int gcpnet_linear_act_forward(const gcp_linear_t* l, const void* resi
         Mat x = {l->x, l->x_ld, l->rows, l->k, 0}, w = {l->w, l->w_ld, l->n, l->k, 0};
         Mat* const both[2] = {&x, &w};
         if (int rc = put_in_pieces<E>(both, 2, workspace, (hipStream_t)stream)) return rc;
-        return product<E>(l->rows, l->n, l->k, x, false, w, false, e, workspace, (hipStream_t)stream);
+        Gemm g;
+        int shape;
+        if (int rc = describe<E>(g, shape, l->rows, l->n, l->k, x, false, w, false, e, workspace)) return rc;
+        return launch<E, false, false>(g, shape, (hipStream_t)stream);
     });
 }
 
@@ -696,14 +739,30 @@ extern "C" int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, 
                 if (const int rc = gcp_column_sums(workspace, (int)by, 1, l->n, &db, &l->bias_type, st)) return rc;
         }
         Epilogue e = {};
+        Gemm one, two;
+        int shape1 = -1, shape2 = -1;
         if (dx && l->rows > 0) {
             e.y = dx;
-            if (int rc = product<E>(l->rows, l->k, l->n, g, false, w, true, e, workspace, st)) return rc;
+            if (int rc = describe<E>(one, shape1, l->rows, l->k, l->n, g, false, w, true, e, workspace)) return rc;
         }
         if (dw) {
             e.y = dw;
-            if (int rc = product<E>(l->n, l->k, l->rows, g, true, x, true, e, workspace, st)) return rc;
+            if (int rc = describe<E>(two, shape2, l->n, l->k, l->rows, g, true, x, true, e, workspace)) return rc;
         }
+        if (shape1 >= 0 && shape1 == shape2 && shape1 < 2) {  // (the largest tiles fill the chip one product at a time)
+            const int64_t groups = (int64_t)one.tiles_m * one.tiles_n * one.splits + (int64_t)two.tiles_m * two.tiles_n * two.splits;
+            by_form(form_of(shape1, groups), [&](auto b, auto wn, auto ring) {
+                constexpr int B = b.value, WN = wn.value;
+                if constexpr (B < 256)
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(gemm_pair_kernel<E, B, B, 2, WN, ring.value>), dim3((unsigned)groups), dim3(128 * WN), 0, st, one, two);
+            });
+            GCP_HIP_CHECK_LAUNCH();
+            if (int rc = join<E>(one, st)) return rc;
+            return join<E>(two, st);
+        }
+        if (shape1 >= 0)
+            if (int rc = launch<E, false, true>(one, shape1, st)) return rc;
+        if (shape2 >= 0) return launch<E, true, true>(two, shape2, st);
         return 0;
     });
 }

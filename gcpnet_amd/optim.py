@@ -4,6 +4,7 @@ of them in one HIP launch per 96 tensors (gcpnet_adam_step) instead of several l
 from __future__ import annotations
 
 import ctypes as C
+import itertools
 from typing import Iterable, Optional
 
 import torch
@@ -140,6 +141,9 @@ class FusedAdam(torch.optim.Optimizer):
         check(lib.gcpnet_adam_step(len(items), arr, float(group["lr"]), float(b1), float(b2), float(group["eps"]),
                                    float(group["weight_decay"]), int(step), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
               "adam_step")
+
+
+_address, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
 
 
 class _Part:
@@ -377,16 +381,15 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _refresh(self, parts, params) -> bool:
         """Whether the same parameters take part with the same state as when `parts` were built; puts this step's gradients in."""
-        grads = [p.grad for p in params]
-        if [id(p) for p, g in zip(params, grads) if g is not None] != self._live(parts):
+        if [id(p) for p in params if p.grad is not None] != self._live(parts):
             return False
         for part in parts:
             ps, dtype = part.params, part.dtype
             grads = [p.grad for p in ps]
-            if ([p.data_ptr() for p in ps] != part.addresses or [g.numel() for g in grads] != part.sizes or any([g.dtype is not dtype for g in grads])
-                    or not all([g.is_contiguous() for g in grads]) or [id(v) for st in part.states for v in st.values()] != part.ids):
+            if (list(map(_address, ps)) != part.addresses or list(map(_numel, grads)) != part.sizes or any([g.dtype is not dtype for g in grads])
+                    or not all(map(_contiguous, grads)) or list(map(id, itertools.chain.from_iterable(map(dict.values, part.states)))) != part.ids):
                 return False
-            pointers = [g.data_ptr() for g in grads]
+            pointers = list(map(_address, grads))
             if pointers != part.grads:
                 for t, g in zip(part.arr, pointers):
                     t.grad = g
@@ -401,7 +404,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _step_device(self, lib, dev, parts):
         stream, where = ops._stream(), torch.device("cuda", dev)
-        corr = torch.empty(2 * sum(len(part.arr) for _, part in parts), dtype=torch.float32, device=where)
+        corr = torch.empty(4 * sum(len(part.arr) for _, part in parts), dtype=torch.float32, device=where)
         clip = partials = None
         count = 0
         if self.max_grad_norm is not None:
@@ -417,7 +420,7 @@ class FusedAdamW(torch.optim.Optimizer):
         at = 0
         for k, (group, part) in enumerate(parts):
             arr = part.arr
-            (b1, b2), lr, here = group["betas"], float(group["lr"]), corr.data_ptr() + 8 * at
+            (b1, b2), lr, here = group["betas"], float(group["lr"]), corr.data_ptr() + 16 * at
             at += len(arr)
             first = clip is not None and k == 0
             check(lib.gcpnet_adamw_begin(len(arr), arr, lr, float(b1), float(b2), here, partials.data_ptr() if first else None, count,

@@ -575,7 +575,7 @@ int gcpnet_adam_step_dev(int n, const gcp_adam_tensor_t* tensors, float lr, floa
  * gcpnet_adamw_step, on one stream; step counts, corrections and the clipping coefficient stay in device memory, so the three may be
  * captured into a hipGraph.  bf16 parameters have an fp32 `master` copy; a parameter that is not the rounding of its master copy (it
  * was written by somebody else) is taken as it is.  `ordinal`, the seed, the step count and an element's index decide the stochastic
- * rounding of exp_avg_sq, so `ordinal` should differ between the tensors of a step.  `vec` is set by the library. */
+ * rounding of exp_avg_sq, so `ordinal` should differ between the tensors of a step.  Any number of tensors per call. */
 typedef struct {
     void* param;
     const void* grad;
@@ -587,15 +587,12 @@ typedef struct {
     float* step;             /* steps taken so far, advanced by gcpnet_adamw_begin */
     int64_t n;
     uint32_t ordinal;
-    int vec;
+    int vec;                 /* the library's own */
 } gcp_adamw_tensor_t;
-#define GCP_ADAMW_MAX_TENSORS 44 /* per launch (any number per call) */
-#define GCP_ADAMW_MAX_BEGIN 448
-#define GCP_ADAMW_MAX_NORM 200
 /* floats that gcpnet_grad_norm writes: sums of squares over 16384 elements each */
 int64_t gcpnet_grad_norm_partials(int n, const gcp_adamw_tensor_t* tensors);
 int gcpnet_grad_norm(int n, const gcp_adamw_tensor_t* tensors, int type, float* partials, void* stream);
-/* step += 1 and corrections[2 k], [2 k + 1] = lr / (1 - beta1^step), 1 / sqrt(1 - beta2^step) for every tensor; with `partials` also
+/* step += 1 and corrections[4 k .. 4 k + 2] = lr / (1 - beta1^step), 1 / sqrt(1 - beta2^step), step for every tensor; with `partials` also
  * clip[0], clip[1] = norm, min(1, max_norm / (norm + 1e-6)) */
 int gcpnet_adamw_begin(int n, const gcp_adamw_tensor_t* tensors, double lr, double beta1, double beta2, float* corrections,
                        const float* partials, int64_t n_partials, float max_norm, float* clip, void* stream);
