@@ -43,23 +43,24 @@ def _wants_grad(tensors) -> bool:
 
 def _rows(t: Tensor) -> Tensor:
     """[..., d] as [rows, d] with unit column stride and any row stride; a copy only where no such view exists."""
-    d = t.shape[-1]
     if t.dim() != 2:
+        d = t.shape[-1]
         try:
             t = t.view(-1, d) if t.numel() else t.reshape(t.numel() // max(d, 1), d)
         except RuntimeError:
             t = t.contiguous().view(-1, d)
-    return t if t.stride(1) == 1 or d == 1 else t.contiguous()
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _check(t, name: str, like: Tensor, shape=None, dtypes=None) -> None:
+def _check(t, name: str, like: Tensor, shape=None, also=None) -> None:
+    """A tensor on like's device, of its type (or `also`) and of the given shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise _lib.GcpnetHipError(f"{name} is on {t.device}, not on {like.device}")
-    if t.dtype not in (dtypes or (like.dtype,)):
-        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes or (like.dtype,))}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if t.dtype is not like.dtype and t.dtype is not also:
+        raise TypeError(f"{name} must be {like.dtype}{'' if also is None else f' or {also}'}, got {t.dtype}")
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
@@ -88,13 +89,10 @@ def _norm_forward(cfg, x, y, gate, weights, need):
     if g2 is not None and not channel and g2.stride(0) == 0 and rows > 1:
         g2 = g2.contiguous()
     ws = [None if w is None else w.contiguous() for w in weights]
-    n = BlockNorm()
-    n.rows, n.d, n.type = rows, d, TYPES[x.dtype]
-    n.param_type = next((TYPES[w.dtype] for w in ws if w is not None), n.type)
-    n.x, n.y, n.gate = x2.data_ptr(), _ptr(y2), _ptr(g2)
-    n.x_ld, n.y_ld, n.gate_ld = x2.stride(0), 0 if y2 is None else y2.stride(0), 0 if g2 is None or channel else d if rows == 1 else g2.stride(0)
-    n.post_w, n.post_b, n.pre_w, n.pre_b = map(_ptr, ws)
-    n.post, n.pre, n.act, n.scale, n.slope, n.eps = NORM[post], NORM[pre], ACT[act], scale, slope, eps
+    kind = TYPES[x.dtype]
+    n = BlockNorm(rows, d, kind, next((TYPES[w.dtype] for w in ws if w is not None), kind), x2.data_ptr(), _ptr(y2), _ptr(g2), x2.stride(0),
+                  0 if y2 is None else y2.stride(0), 0 if g2 is None or channel else d if rows == 1 else g2.stride(0), *map(_ptr, ws), NORM[post],
+                  NORM[pre], ACT[act], scale, slope, eps)
     with _on(x):
         s = x.new_empty(x.shape) if y is not None else None
         h = x.new_empty(x.shape) if pre is not None else None
@@ -111,14 +109,10 @@ def _norm_backward(ctx, ds, dh):
         return (None,) * 8
     ds, dh = (None if g is None else g.contiguous() for g in (ds, dh))
     _, need_x, need_y, need_gate, *need_w = ctx.needs_input_grad
-    b = BlockNorm.from_buffer_copy(n)  # (addresses anew: what was saved may have been elsewhere meanwhile)
-    b.x, b.x_ld = None, n.d if y2 is not None else s.stride(0)
-    b.y, b.gate = _ptr(y2), _ptr(g2)
-    b.post_w, b.post_b, b.pre_w, b.pre_b = map(_ptr, ws)
-    if y2 is not None:
-        b.y_ld = y2.stride(0)
-    if g2 is not None and not ctx.channel and n.rows > 1:
-        b.gate_ld = g2.stride(0)
+    # (addresses anew: what was saved may have been elsewhere meanwhile)
+    b = BlockNorm(n.rows, n.d, n.type, n.param_type, None, _ptr(y2), _ptr(g2), n.d if y2 is not None else s.stride(0),
+                  0 if y2 is None else y2.stride(0), 0 if g2 is None or ctx.channel else n.d if n.rows == 1 else g2.stride(0), *map(_ptr, ws), n.post,
+                  n.pre, n.act, n.scale, n.slope, n.eps)
     lib = _lib.load()
     new = lambda want, like: s.new_empty(like) if want else None  # noqa: E731
     dx, dy = new(need_x, shape), new(need_y and y2 is not None, shape)
@@ -191,8 +185,10 @@ def residual_norm(x: Tensor, y: Optional[Tensor] = None, gate: Optional[Tensor] 
             continue
         if kind is None:
             raise ValueError(f"residual_norm: {name} without its norm")
-        _check(w, name, x, (d,), (x.dtype, torch.float32) if first is None else (first,))
-        first = w.dtype
+        _check(w, name, x, (d,), torch.float32)
+        first = first or w.dtype
+        if w.dtype is not first:
+            raise TypeError(f"residual_norm: weights and biases of one type, got {first} and {w.dtype}")
     cfg, weights = (post, pre, gate_act, float(scale), float(slope), float(eps)), (post_weight, post_bias, pre_weight, pre_bias)
     if _wants_grad((x, y, gate, *weights)):
         s, h = _ResidualNorm.apply(cfg, x, y, gate, *weights)
@@ -211,10 +207,9 @@ def _linear_forward(cfg, x, weight, bias, residual, need):
     b2 = None if bias is None else bias.contiguous()
     rows, k = x2.shape
     n = w2.shape[0]
-    q = LinearDesc()
-    q.rows, q.k, q.n, q.type, q.act, q.slope = rows, k, n, TYPES[x.dtype], ACT[act], slope
-    q.bias_type = q.type if b2 is None else TYPES[b2.dtype]
-    q.x, q.w, q.bias, q.x_ld, q.w_ld = x2.data_ptr(), w2.data_ptr(), _ptr(b2), x2.stride(0), w2.stride(0)
+    kind = TYPES[x.dtype]
+    q = LinearDesc(rows, k, n, kind, kind if b2 is None else TYPES[b2.dtype], ACT[act], slope, x2.data_ptr(), w2.data_ptr(), _ptr(b2), x2.stride(0),
+                   w2.stride(0))
     lib = _lib.load()
     with _on(x):
         y = x.new_empty((*x.shape[:-1], n))
@@ -231,8 +226,8 @@ def _linear_backward(ctx, dy):
     if not (need_x or need_w or need_b):
         return None, None, None, None, dy if need_r else None
     x2, w2, z = ctx.saved_tensors
-    q = LinearDesc.from_buffer_copy(ctx.desc)  # (addresses anew: what was saved may have been elsewhere meanwhile)
-    q.x, q.w, q.bias, q.x_ld, q.w_ld = x2.data_ptr(), w2.data_ptr(), None, x2.stride(0), w2.stride(0)
+    d = ctx.desc  # (its addresses anew: what was saved may have been elsewhere meanwhile)
+    q = LinearDesc(d.rows, d.k, d.n, d.type, d.bias_type, d.act, d.slope, x2.data_ptr(), w2.data_ptr(), None, x2.stride(0), w2.stride(0))
     g2 = _rows(dy)
     lib = _lib.load()
     dx = x2.new_empty(ctx.shapes[0]) if need_x else None
@@ -272,7 +267,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Op
         raise ValueError(f"linear_act: act is None or one of {sorted(k for k in ACT if k)}, got {act!r}")
     n = weight.shape[0]
     if bias is not None:
-        _check(bias, "bias", x, (n,), (x.dtype, torch.float32))
+        _check(bias, "bias", x, (n,), torch.float32)
     if residual is not None:
         _check(residual, "residual", x, (*x.shape[:-1], n))
     if _wants_grad((x, weight, bias, residual)):
