@@ -9,7 +9,9 @@
 //   * tiles of 128 bytes of k travel from memory into a ring of LDS buffers by direct loads (no registers); the 16-byte pieces of an LDS
 //     row are permuted (by the row) so that fragment reads spread over the banks;
 //   * a tile is two steps of the 16-bit matrix instructions; while one step's fragments are multiplied the next step's are read, B's into
-//     a second set of registers, A's into the registers of the row of products just issued; the waves meet once a tile;
+//     a second set of registers, A's into the registers of the row of products just issued; the waves meet once a tile, and the direct loads
+//     of the next free buffer are spread between the rows of products (all at once they held the matrix pipe up: 8192 x 4096 x 4096 bf16
+//     240 us, spread 223.5 = 1.23 PFLOP/s);
 //   * an operand with k across memory keeps its layout in LDS, [k][m]; 16-bit fragments come out of it through the transposing LDS
 //     read, fp32 ones element by element;
 //   * operands whose rows are not whole 16-byte pieces are first copied into the workspace, rows filled up with zeros (one launch for all of
@@ -118,20 +120,17 @@ struct Tile {
         else return (unsigned)((row * ld + (piece * PE < left ? piece * PE : left - PE)) * S);
     }
 
-    // the tile from memory; `left`: k from its start on
+    // turn t of the tile from memory; WHOLE: k does not end in it, else `left` is k from its start on
     template <bool WHOLE>
-    __device__ static __forceinline__ void stage(char* lds, const char* from, const unsigned (&offsets)[TURNS], int64_t left) {
+    __device__ static __forceinline__ void stage(char* lds, const char* from, unsigned offset, int t, int64_t left) {
         const int wave = threadIdx.x >> 6;
-#pragma unroll
-        for (int t = 0; t < TURNS; ++t) {
-            if constexpr (WHOLE) {
-                to_lds(from, offsets[t], lds + (t * THREADS + wave * 64) * 16);
-            } else {
-                int row, piece;
-                where(t * THREADS + (int)threadIdx.x, row, piece);
-                if ((ACROSS ? row : piece * PE) < left) to_lds(from, offsets[t], lds + (t * THREADS + wave * 64) * 16);
-                else *(u32x4*)(lds + (t * THREADS + (int)threadIdx.x) * 16) = u32x4{0, 0, 0, 0};
-            }
+        if constexpr (WHOLE) {
+            to_lds(from, offset, lds + (t * THREADS + wave * 64) * 16);
+        } else {
+            int row, piece;
+            where(t * THREADS + (int)threadIdx.x, row, piece);
+            if ((ACROSS ? row : piece * PE) < left) to_lds(from, offset, lds + (t * THREADS + wave * 64) * 16);
+            else *(u32x4*)(lds + (t * THREADS + (int)threadIdx.x) * 16) = u32x4{0, 0, 0, 0};
         }
     }
 
@@ -209,14 +208,17 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, int block, int piece, c
     const int64_t da = (AC ? g.a_ld * TA::KE : TA::KE) * TA::S, db = (BC ? g.b_ld * TB::KE : TB::KE) * TB::S;
 
     auto stage = [&](int step, char* buf) {
-        const char *fa = pa + step * da, *fb = pb + step * db;
         if (step < whole) {
-            TA::template stage<true>(buf, fa, oa, 0);
-            TB::template stage<true>(buf + TA::BYTES, fb, ob, 0);
+#pragma unroll
+            for (int t = 0; t < TA::TURNS; ++t) TA::template stage<true>(buf, pa + step * da, oa[t], t, 0);
+#pragma unroll
+            for (int t = 0; t < TB::TURNS; ++t) TB::template stage<true>(buf + TA::BYTES, pb + step * db, ob[t], t, 0);
         } else {
             const int64_t left = k1 - k0 - (int64_t)step * TA::KE;
-            TA::template stage<false>(buf, fa, oa, left);
-            TB::template stage<false>(buf + TA::BYTES, fb, ob, left);
+#pragma unroll
+            for (int t = 0; t < TA::TURNS; ++t) TA::template stage<false>(buf, pa + step * da, oa[t], t, left);
+#pragma unroll
+            for (int t = 0; t < TB::TURNS; ++t) TB::template stage<false>(buf + TA::BYTES, pb + step * db, ob[t], t, left);
         }
     };
 
@@ -231,7 +233,8 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, int block, int piece, c
         for (int j = 0; j < TN; ++j) fb[kk][j] = TB::fragment(buf + TA::BYTES, (wn * TN + j) * 16, kk, lane);
     };
     auto read_a = [&](const char* buf, int kk, int i) { fa[i] = TA::fragment(buf, (wm * TM + i) * 16, kk, lane); };
-    auto multiply = [&](auto kk, const char* buf, int then) {  // the products of step kk; fragments of A for step `then` of buf
+    // the products of step kk; meanwhile fragments of A for step `then` of buf and, between the rows of products, the direct loads of tile `ahead`
+    auto multiply = [&](auto kk, const char* buf, int then, auto loads, int ahead, char* into) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             __builtin_amdgcn_sched_barrier(0);
@@ -239,6 +242,12 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, int block, int piece, c
             for (int j = 0; j < TN; ++j) acc[i][j] = mfma<E>(fb[kk][j], fa[i], acc[i][j]);  // (transposed: a lane gets four n of one m)
             __builtin_amdgcn_sched_barrier(0);  // (not before: the registers are the products')
             read_a(buf, then, i);
+            if constexpr (decltype(loads)::value) {
+#pragma unroll
+                for (int t = i * TA::TURNS / TM; t < (i + 1) * TA::TURNS / TM; ++t) TA::template stage<true>(into, pa + ahead * da, oa[t], t, 0);
+#pragma unroll
+                for (int t = i * TB::TURNS / TM; t < (i + 1) * TB::TURNS / TM; ++t) TB::template stage<true>(into + TA::BYTES, pb + ahead * db, ob[t], t, 0);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -252,19 +261,28 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, int block, int piece, c
     read_b(buf, first);
 #pragma unroll
     for (int i = 0; i < TM; ++i) read_a(buf, 0, i);
-#pragma unroll 1
-    for (int s = 0; s < steps; ++s) {
+    auto turn = [&](int s, auto ahead) {  // ahead: the tile that follows the ring is whole
         char* next = buf + STAGE == lds + RING * STAGE ? lds : buf + STAGE;
         read_b(buf, second);
-        multiply(first, buf, 1);
+        multiply(first, buf, 1, std::false_type(), 0, nullptr);
         // everybody has all of this tile's fragments, and the next tile is there: those after it may still be under way
-        if (s + RING <= whole) wait_loads_and_meet<(RING - 2) * LOADS>();
-        else wait_loads_and_meet<0>();
+        if constexpr (decltype(ahead)::value) {
+            wait_loads_and_meet<(RING - 2) * LOADS>();
+        } else {
+            if (s + RING <= whole) wait_loads_and_meet<(RING - 2) * LOADS>();
+            else wait_loads_and_meet<0>();
+        }
         read_b(next, first);  // (behind the last tile: what is there is read, and not used)
-        if (s + RING < steps) stage(s + RING, buf);
-        multiply(second, next, 0);
+        if constexpr (!decltype(ahead)::value)
+            if (s + RING < steps) stage(s + RING, buf);
+        multiply(second, next, 0, ahead, s + RING, buf);
         buf = next;
-    }
+    };
+    int s = 0;
+#pragma unroll 1
+    for (; s + RING < whole; ++s) turn(s, std::true_type());
+#pragma unroll 1
+    for (; s < steps; ++s) turn(s, std::false_type());
     __syncthreads();  // (the epilogue writes over the ring)
 
     // A wave's part of C goes through its own LDS, PH rows at a time: [PH][COLS] fp32 in pieces of 16 bytes, piece p of row r at p ^ (r & mask)
