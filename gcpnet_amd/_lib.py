@@ -265,7 +265,7 @@ def load():
     lib.gcpnet_adamw_begin.argtypes = [i32, AW, f64, f64, f64, vp, vp, i64, f32, vp, vp]
     lib.gcpnet_adamw_step.argtypes = [i32, AW, i32, i32, f64, f64, f64, f64, f64, vp, vp, C.c_uint32, vp]
     lib.gcpnet_block_norm_forward.argtypes = [P(BlockNorm), vp, vp, vp, vp]
-    lib.gcpnet_block_norm_backward.argtypes = [P(BlockNorm)] + [vp] * 13
+    lib.gcpnet_block_norm_backward.argtypes = [P(BlockNorm)] + [vp] * 12
     lib.gcpnet_block_norm_backward_scratch.argtypes = [P(BlockNorm)]
     lib.gcpnet_block_norm_backward_scratch.restype = i64
     lib.gcpnet_linear_act_workspace.argtypes = [P(LinearDesc), i32]

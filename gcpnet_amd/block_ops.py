@@ -98,32 +98,33 @@ def _norm_forward(cfg, x, y, gate, weights, need):
         h = x.new_empty(x.shape) if pre is not None else None
         stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if need and (post or pre) else None
         check(_lib.load().gcpnet_block_norm_forward(C.byref(n), _ptr(s), _ptr(h), _ptr(stats), _stream()), "residual_norm")
-    return s, h, (n, channel, (y2, s if s is not None else x2, g2, stats, *ws))
+    return s, h, (n, channel, (x2 if pre else None, y2, g2, stats, *ws))
 
 
 def _norm_backward(ctx, ds, dh):
-    y2, s, g2, stats, *ws = ctx.saved_tensors
+    x2, y2, g2, stats, *ws = ctx.saved_tensors
     shape, gate_shape = ctx.shapes
     n = ctx.desc
     if ds is None and dh is None:
         return (None,) * 8
     ds, dh = (None if g is None else g.contiguous() for g in (ds, dh))
+    like = dh if ds is None else ds
     _, need_x, need_y, need_gate, *need_w = ctx.needs_input_grad
     # (addresses anew: what was saved may have been elsewhere meanwhile)
-    b = BlockNorm(n.rows, n.d, n.type, n.param_type, None, _ptr(y2), _ptr(g2), n.d if y2 is not None else s.stride(0),
-                  0 if y2 is None else y2.stride(0), 0 if g2 is None or ctx.channel else n.d if n.rows == 1 else g2.stride(0), *map(_ptr, ws), n.post,
-                  n.pre, n.act, n.scale, n.slope, n.eps)
+    b = BlockNorm(n.rows, n.d, n.type, n.param_type, _ptr(x2), _ptr(y2), _ptr(g2), 0 if x2 is None else x2.stride(0), 0 if y2 is None else y2.stride(0),
+                  0 if g2 is None or ctx.channel else n.d if n.rows == 1 else g2.stride(0), *map(_ptr, ws), n.post, n.pre, n.act, n.scale, n.slope,
+                  n.eps)
     lib = _lib.load()
-    new = lambda want, like: s.new_empty(like) if want else None  # noqa: E731
+    new = lambda want, size: like.new_empty(size) if want else None  # noqa: E731
     dx, dy = new(need_x, shape), new(need_y and y2 is not None, shape)
     need_gate = need_gate and g2 is not None
     dgate = new(need_gate and not ctx.channel, gate_shape)
     dws = [None] * 4
     wanted = [i for i in range(4) if need_w[i] and ws[i] is not None]
-    dtype = ws[wanted[0]].dtype if wanted else s.dtype
-    together = need_gate and ctx.channel and dtype == s.dtype  # (one allocation for the short ones)
+    dtype = ws[wanted[0]].dtype if wanted else like.dtype
+    together = need_gate and ctx.channel and dtype == like.dtype  # (one allocation for the short ones)
     if wanted or together:
-        short = iter(s.new_empty((len(wanted) + together, n.d), dtype=dtype).unbind())
+        short = iter(like.new_empty((len(wanted) + together, n.d), dtype=dtype).unbind())
         for i in wanted:
             dws[i] = next(short)
         if together:
@@ -132,8 +133,8 @@ def _norm_backward(ctx, ds, dh):
         dgate = new(True, gate_shape)
     scratch = None
     if wanted or (dgate is not None and ctx.channel):
-        scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(C.byref(b)))), dtype=torch.float32, device=s.device)
-    check(lib.gcpnet_block_norm_backward(C.byref(b), s.data_ptr(), _ptr(stats), _ptr(ds), _ptr(dh), _ptr(dx), _ptr(dy), _ptr(dgate),
+        scratch = torch.empty(max(1, int(lib.gcpnet_block_norm_backward_scratch(C.byref(b)))), dtype=torch.float32, device=like.device)
+    check(lib.gcpnet_block_norm_backward(C.byref(b), _ptr(stats), _ptr(ds), _ptr(dh), _ptr(dx), _ptr(dy), _ptr(dgate),
                                          *map(_ptr, dws), _ptr(scratch), _stream()), "residual_norm backward")
     return (None, dx, dy, dgate, *dws)
 

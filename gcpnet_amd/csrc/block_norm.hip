@@ -6,7 +6,8 @@
 //   dx = gs;  du = scale act(gate) gs;  dgate = scale gs u act'(gate);  dy = rstd1 (du w - mean(du w) - n1 mean(du w n1))
 //   weights and biases: column sums of dh n2, dh, du n1, du, and of dgate for a gate of one value per channel.
 //
-// Bound: HBM -- forward reads x, y (and an element-wise gate) and writes s, h; backward reads y, s, ds, dh, writes dx, dy.  A row is
+// Bound: HBM -- forward reads x, y (and an element-wise gate) and writes s, h; backward reads x, y, ds, dh, writes dx, dy (s is formed again
+// from x as the forward formed it, unrounded, for the same bytes that reading it would take).  A row is
 // held in the registers of a group of 8 to 1024 threads between its reductions, so everything is read once; the statistics take
 // two passes over the registers (mean, then squares of the differences).  The backward's groups walk many rows and keep the column sums
 // in registers; one partial sum per workgroup goes through memory, summed in a fixed order by a second launch.
@@ -158,12 +159,19 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
     if (a.stats && on && t == 0) *(f32x4*)(a.stats + 4 * r) = f32x4{st[0], st[1], st[2], st[3]};
 }
 
+// Waves per SIMD that the backward's registers leave room for; its workgroups are counted by them.
+template <class E, int G, int NV>
+constexpr int backward_waves() { return G > 512 ? 4 : NV > 1 ? 2 : E::vec == 8 ? 3 : 4; }
+
 // BIAS: with the sums of the biases and of a gate of one value per channel, too.  Those lie in LDS, where each thread adds to places of its
 // own: in registers they would take the room of the row that is requested ahead.
 template <class E, int G, int NV, bool BIAS>
 __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a) {
     constexpr int V = E::vec;
     constexpr int PER = (G > 256 ? G : 256) / G;
+    // A gate's sigmoid is kept between its two uses where two workgroups a CU leave registers for it (16384 x 4096 bf16, both
+    // directions: 407 us against 418), and formed twice where three are to fit (60000 x 1000 fp16, backward: 275 us against 286).
+    constexpr bool KEEP = NV > 1;
     __shared__ float lds[2][2][16];
     __shared__ float cols[PER > 1 ? 256 * NV * V : 1];
     int turn = 0;
@@ -195,8 +203,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[q][k][j] = 0.f;
-    const bool channel = a.gate && a.gate_ld == 0;
-    struct Row { Raw<E, V> y[NV], s[NV], g[NV], ds[NV], dh[NV]; f32x4 st; };
+    const bool channel = a.gate && a.gate_ld == 0, full = KEEP && a.d == G * NV * V;  // (full: no thread has less than its vectors)
+    struct Row { Raw<E, V> x[NV], y[NV], g[NV], ds[NV], dh[NV]; f32x4 st; };
     auto request = [&](int64_t first, Row& q) {
         const int64_t r = first + threadIdx.x / G;
         const bool on = r < a.rows;
@@ -206,7 +214,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
         for (int k = 0; k < NV; ++k) {
             const int c = (k * G + t) * V, n = on ? in[k] : 0;
             q.y[k] = a.y ? elem_load<E, V>(a.y, r * a.y_ld + c, n) : elem_zero<E, V>();
-            q.s[k] = a.pre ? elem_load<E, V>(a.s, r * a.x_ld + c, n) : elem_zero<E, V>();
+            q.x[k] = a.pre ? elem_load<E, V>(a.x, r * a.x_ld + c, n) : elem_zero<E, V>();
             q.g[k] = a.gate ? elem_load<E, V>(a.gate, r * a.gate_ld + c, n) : elem_zero<E, V>();
             q.ds[k] = a.ds ? elem_load<E, V>(a.ds, r * a.d + c, n) : elem_zero<E, V>();
             q.dh[k] = a.dh ? elem_load<E, V>(a.dh, r * a.d + c, n) : elem_zero<E, V>();
@@ -229,29 +237,56 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
         } else {
             request(first, now);
         }
-        const auto &yr = now.y, &sr = now.s, &gr = now.g, &dsr = now.ds, &dhr = now.dh;
+        const auto &xr = now.x, &yr = now.y, &gr = now.g, &dsr = now.ds, &dhr = now.dh;
         const f32x4 st = now.st;
-        float gs[NV][V];
+        float gs[NV][V], sig[KEEP ? NV : 1][V];
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) gs[k][j] = dsr[k][j];
+        if (KEEP && a.gate && elem_by_sigmoid(a.act))
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) sig[k][j] = elem_sigmoid(gr[k][j]);
         if (a.dh) {
-            float m[2] = {0.f, 0.f}, dn[NV][V];
+            float m[2] = {0.f, 0.f}, n2[NV][V], dn[NV][V];
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
+                const int c = (k * G + t) * V;
+                if (a.y) {  // s, as in the forward
+                    float u[V], g[V], none[V], w[V], b[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; g[j] = gr[k][j]; u[j] = yr[k][j]; }
+                    if (a.post) {
+                        param_load<E, V>(a.post_w, c, in[k], a.w_f32, w);
+                        param_load<E, V>(a.post_b, c, in[k], a.w_f32, b);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) u[j] = fmaf((u[j] - st[0]) * st[1], w[j], b[j]);
+                    }
+                    if (a.gate) {
+                        if constexpr (KEEP) elem_act_with<V, false>(a.act, a.slope, g, sig[k], g, none);
+                        else elem_act<V, false>(a.act, a.slope, g, g, none);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) u[j] *= g[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < V; ++j) n2[k][j] = (fmaf(a.scale, u[j], xr[k][j]) - st[2]) * st[3];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) n2[k][j] = (xr[k][j] - st[2]) * st[3];
+                }
                 float w[V], d[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) w[j] = 1.f;
-                param_load<E, V>(a.pre_w, (k * G + t) * V, in[k], a.w_f32, w);
+                param_load<E, V>(a.pre_w, c, in[k], a.w_f32, w);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float dh = dhr[k][j], n = (sr[k][j] - st[2]) * st[3];
-                    dn[k][j] = dh * w[j];  // (0 outside)
+                    d[j] = dhr[k][j];  // (0 outside)
+                    dn[k][j] = d[j] * w[j];
                     m[0] += dn[k][j];
-                    m[1] = fmaf(dn[k][j], n, m[1]);
-                    sum[0][k][j] = fmaf(dh, n, sum[0][k][j]);
-                    d[j] = dh;
+                    m[1] = fmaf(dn[k][j], n2[k][j], m[1]);
+                    sum[0][k][j] = fmaf(d[j], n2[k][j], sum[0][k][j]);
                 }
                 if constexpr (BIAS)
                     if (a.slot[2] >= 0) add(2, k, d);
@@ -261,10 +296,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
 #pragma unroll
             for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float n = (sr[k][j] - st[2]) * st[3];
-                    gs[k][j] = fmaf(st[3], fmaf(-n, m1, dn[k][j] - m0), gs[k][j]);
-                }
+                for (int j = 0; j < V; ++j) gs[k][j] = fmaf(st[3], fmaf(-n2[k][j], m1, dn[k][j] - m0), gs[k][j]);
         }
         if (a.dx)
 #pragma unroll
@@ -283,13 +315,14 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 n[j] = (yr[k][j] - st[0]) * st[1];
-                gs[k][j] = j < in[k] && on ? gs[k][j] * a.scale : 0.f;
+                gs[k][j] = full || j < in[k] ? gs[k][j] * a.scale : 0.f;
             }
             if (a.gate) {
                 float g[V], da[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) g[j] = gr[k][j];
-                elem_act<V, true>(a.act, a.slope, g, g, da);
+                if constexpr (KEEP) elem_act_with<V, true>(a.act, a.slope, g, sig[k], g, da);
+                else elem_act<V, true>(a.act, a.slope, g, g, da);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float u = a.post ? fmaf(n[j], w[j], b[j]) : yr[k][j];
@@ -401,7 +434,7 @@ bool by_shape(int d, F f) {
 // them than CUs (the partial sums of each have to be added).
 template <class E, int G, int NV>
 int64_t backward_blocks(int64_t rows) {
-    constexpr int T = G > 256 ? G : 256, most = T > 256 ? 256 : NV > 1 ? 512 : E::vec == 8 ? 768 : 1024;
+    constexpr int T = G > 256 ? G : 256, most = 256 * (backward_waves<E, G, NV>() * 256 / T);
     const int64_t blocks = (rows + T / G - 1) / (T / G), few = blocks < 256 ? blocks : blocks < 1024 ? 256 : blocks / 4;
     return few < most ? few : most;
 }
@@ -479,12 +512,12 @@ extern "C" int64_t gcpnet_block_norm_backward_scratch(const gcp_block_norm_t* n)
     return blocks * SETS * n->d;
 }
 
-extern "C" int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const void* s, const float* stats, const void* ds, const void* dh,
+extern "C" int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const float* stats, const void* ds, const void* dh,
                                           void* dx, void* dy, void* dgate, void* d_post_w, void* d_post_b, void* d_pre_w, void* d_pre_b,
                                           float* scratch, void* stream) {
     if (int rc = check_desc(n)) return rc;
     if ((n->post || n->pre) && n->rows > 0 && (!stats || !aligned16(stats))) return GCPNET_E_BADARG;
-    if (n->rows > 0 && n->pre && dh && !s) return GCPNET_E_BADARG;
+    if (n->rows > 0 && n->pre && dh && !n->x) return GCPNET_E_BADARG;
     NormArgs a = fill(n);
     const bool channel = n->gate && n->gate_ld == 0;
     void* const out[SETS] = {n->pre ? d_pre_w : nullptr, n->post ? d_post_w : nullptr, n->pre ? d_pre_b : nullptr, n->post ? d_post_b : nullptr,
@@ -500,7 +533,6 @@ extern "C" int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const void*
     if (a.sets && n->rows > 0 && !scratch) return GCPNET_E_BADARG;
     int64_t blocks = 0;
     if (n->rows > 0) {
-        a.s = const_cast<void*>(s);
         a.pre = n->pre && dh ? n->pre : 0;
         a.dh = n->pre ? dh : nullptr;
         a.ds = ds; a.dx = dx; a.dy = dy; a.dgate = dgate;

@@ -78,17 +78,21 @@ __device__ __forceinline__ void param_load(const void* base, int64_t at, int cou
     }
 }
 
-// act(v), and with GRAD also act'(v), of V values; the choice is uniform and made once for all of them.  The sigmoid's reciprocal is the
-// hardware's, good to a unit in the last place of fp32.
+// The sigmoid by the hardware's reciprocal, good to a unit in the last place of fp32.
+__device__ __forceinline__ float elem_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
+__device__ __forceinline__ bool elem_by_sigmoid(int act) { return act == GCP_ACT_SILU || act == GCP_ACT_SIGMOID; }
+
+// act(v), and with GRAD also act'(v), of V values; the choice is uniform and made once for all of them.  `s`: the sigmoids of v where the
+// activation is made of them (else not looked at).
 template <int V, bool GRAD>
-__device__ __forceinline__ void elem_act(int act, float slope, const float (&v)[V], float (&a)[V], float (&d)[V]) {
-    if (act == GCP_ACT_SILU || act == GCP_ACT_SIGMOID) {
+__device__ __forceinline__ void elem_act_with(int act, float slope, const float (&v)[V], const float (&s)[V], float (&a)[V], float (&d)[V]) {
+    if (elem_by_sigmoid(act)) {
         const bool silu = act == GCP_ACT_SILU;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float x = v[j], s = __builtin_amdgcn_rcpf(1.f + __expf(-x)), r = s * (1.f - s);
-            a[j] = silu ? x * s : s;
-            if constexpr (GRAD) d[j] = silu ? fmaf(x, r, s) : r;
+            const float x = v[j], r = s[j] * (1.f - s[j]);
+            a[j] = silu ? x * s[j] : s[j];
+            if constexpr (GRAD) d[j] = silu ? fmaf(x, r, s[j]) : r;
         }
     } else if (act == GCP_ACT_SELU) {
 #pragma unroll
@@ -106,6 +110,14 @@ __device__ __forceinline__ void elem_act(int act, float slope, const float (&v)[
             if constexpr (GRAD) d[j] = x > 0.f ? 1.f : low;
         }
     }
+}
+template <int V, bool GRAD>
+__device__ __forceinline__ void elem_act(int act, float slope, const float (&v)[V], float (&a)[V], float (&d)[V]) {
+    float s[V];
+    if (elem_by_sigmoid(act))
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = elem_sigmoid(v[j]);
+    elem_act_with<V, GRAD>(act, slope, v, s, a, d);
 }
 
 inline bool elem_type_ok(int t) { return t == GCP_TYPE_F32 || t == GCP_TYPE_BF16 || t == GCP_TYPE_F16; }

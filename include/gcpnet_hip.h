@@ -634,11 +634,10 @@ typedef struct {
     float scale, slope, eps;
 } gcp_block_norm_t;
 int gcpnet_block_norm_forward(const gcp_block_norm_t* n, void* s, void* h, float* stats, void* stream);
-/* s: the forward's output s with row stride x_ld (the forward's x itself where y was NULL); ds, dh contiguous or NULL (= 0); outputs contiguous,
- * each may be NULL; dgate is [rows, d], or [d] with gate_ld 0.  Column sums are formed in a fixed order.  scratch:
- * gcpnet_block_norm_backward_scratch(n) floats. */
+/* The descriptor of the forward, with x, y, gate as they were; ds, dh contiguous or NULL (= 0); outputs contiguous, each may be NULL; dgate is
+ * [rows, d], or [d] with gate_ld 0.  Column sums are formed in a fixed order.  scratch: gcpnet_block_norm_backward_scratch(n) floats. */
 int64_t gcpnet_block_norm_backward_scratch(const gcp_block_norm_t* n);
-int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const void* s, const float* stats, const void* ds, const void* dh, void* dx,
+int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const float* stats, const void* ds, const void* dh, void* dx,
                                void* dy, void* dgate, void* d_post_w, void* d_post_b, void* d_pre_w, void* d_pre_b, float* scratch,
                                void* stream);
 

@@ -73,7 +73,6 @@ def reference(cfg, t, x, y, gate, pw, pb, qw, qb, ds, dh, scale, eps):
 
     gs, d_gs = ds, 0 * ds
     if pre:
-        d_n2 = d_n2 + (half(t) * s.abs() * r2 if t != torch.float32 else 0)  # (the backward reads the stored s)
         dn = dh * w2
         m0, m1 = (dn.mean(1, keepdim=True) if pre == "layer" else 0), (dn * n2).mean(1, keepdim=True)
         d_m1 = (dn.abs() * d_n2).mean(1, keepdim=True) + e * (dn * n2).abs().mean(1, keepdim=True)
@@ -363,7 +362,7 @@ def test_refusals():
         setattr(n, field, keep)
     n.pre = 1
     assert lib.gcpnet_block_norm_forward(n, None, None, None, None) == -1  # (pre without h)
-    assert lib.gcpnet_block_norm_backward(n, 4096, None, *[None] * 11) == -1  # (pre without statistics)
+    assert lib.gcpnet_block_norm_backward(n, None, *[None] * 11) == -1  # (pre without statistics)
     n.rows = 0
     assert call() == 0
     n.rows = -1
