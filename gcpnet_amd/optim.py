@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes as C
 import itertools
+import operator
 from typing import Iterable, Optional
 
 import torch
@@ -144,6 +145,7 @@ class FusedAdam(torch.optim.Optimizer):
 
 
 _address, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_grad, _dtype = operator.attrgetter("grad"), operator.attrgetter("dtype")
 
 
 class _Part:
@@ -155,11 +157,11 @@ class _Part:
         self.params = [p for p, _, _, _ in items]
         self.arr = (AdamWTensor * len(items))()
         self.copies = []
-        # what the next step compares with (strong references: an id stays its object's); a permuted parameter never matches, its table is
-        # built anew every step
+        # what the next step compares with (the tensors of the state are kept alive, so that their addresses stay theirs); a permuted parameter
+        # or a state that holds something else than tensors never matches: such a table is built anew every step
         self.states = [st for _, _, st, _ in items]
         self.held = [v for st in self.states for v in st.values()]
-        self.ids = [id(v) for v in self.held]
+        self.where = [v.data_ptr() for v in self.held] if all(map(torch.is_tensor, self.held)) else None
         self.live, self.order = [id(p) for p in self.params], [ordinal for _, _, _, ordinal in items]
         self.addresses = [p.data_ptr() if p.is_contiguous() else None for p in self.params]
         self.sizes = [p.numel() for p in self.params]
@@ -225,6 +227,8 @@ class FusedAdamW(torch.optim.Optimizer):
     @classmethod
     def _check_group(cls, g):
         cls._check_options(g)
+        if len(set(map(id, g["params"]))) != len(g["params"]):
+            raise ValueError("FusedAdamW: a parameter twice in one group (both updates would run at once)")
         for p in g["params"]:
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError(f"FusedAdamW: fp32 and bf16 parameters only, got {p.dtype}")
@@ -377,23 +381,36 @@ class FusedAdamW(torch.optim.Optimizer):
                 else:
                     self._check_state(p, st, bits)
                 parts.setdefault((p.device.index, p.dtype), []).append((p, g, st, ordinal + k))
+        for items in parts.values():  # (the updates of a launch run at once)
+            end = 0
+            for start, size in sorted((p.data_ptr(), p.numel() * p.element_size()) for p, _, _, _ in items if p.numel()):
+                if start < end:
+                    raise _lib.GcpnetHipError("FusedAdamW: parameters of one group must not share memory")
+                end = start + size
         return [_Part(dev, dtype, items, bits) for (dev, dtype), items in parts.items()]
 
     def _refresh(self, parts, params) -> bool:
         """Whether the same parameters take part with the same state as when `parts` were built; puts this step's gradients in."""
-        if [id(p) for p in params if p.grad is not None] != self._live(parts):
-            return False
-        for part in parts:
-            ps, dtype = part.params, part.dtype
-            grads = [p.grad for p in ps]
-            if (list(map(_address, ps)) != part.addresses or list(map(_numel, grads)) != part.sizes or any([g.dtype is not dtype for g in grads])
-                    or not all(map(_contiguous, grads)) or list(map(id, itertools.chain.from_iterable(map(dict.values, part.states)))) != part.ids):
+        try:
+            if len(parts) == 1 and list(map(id, params)) == parts[0].live:
+                return self._same(parts[0], list(map(_grad, params)))
+            if [id(p) for p in params if p.grad is not None] != self._live(parts):
                 return False
-            pointers = list(map(_address, grads))
-            if pointers != part.grads:
-                for t, g in zip(part.arr, pointers):
-                    t.grad = g
-                part.grads = pointers
+            return all([self._same(part, list(map(_grad, part.params))) for part in parts])
+        except TypeError:  # (something is not a tensor: a gradient that is None, a value put into a state)
+            return False
+
+    @staticmethod
+    def _same(part, grads) -> bool:
+        if (part.where is None or list(map(_address, part.params)) != part.addresses or list(map(_numel, part.params)) != part.sizes
+                or list(map(_numel, grads)) != part.sizes or set(map(_dtype, grads)) != {part.dtype} or not all(map(_contiguous, grads))
+                or list(map(_address, itertools.chain.from_iterable(map(dict.values, part.states)))) != part.where):
+            return False
+        pointers = list(map(_address, grads))
+        if pointers != part.grads:
+            for t, g in zip(part.arr, pointers):
+                t.grad = g
+            part.grads = pointers
         return True
 
     @staticmethod

@@ -119,6 +119,12 @@ def test_refusals():
         opt.step()
 
 
+def test_a_parameter_twice_is_refused():
+    w = torch.nn.Parameter(torch.zeros(3))
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="twice"):
+        G.FusedAdamW([w, w])
+
+
 def test_bad_arguments_at_the_c_entries():
     lib = _lib.load()
     arr = (_lib.AdamWTensor * 1)()
@@ -454,3 +460,41 @@ def test_more_than_2_to_the_32_elements():
     assert float(st["master"][:1 << 20].abs().max()) == 0.0
     del p, opt, st
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_shared_memory_is_refused():
+    a = torch.nn.Parameter(torch.zeros(600, device="cuda"))
+    b = torch.nn.Parameter(a.detach()[300:])
+    c = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    with pytest.raises(_lib.GcpnetHipError, match="share memory"):
+        G.FusedAdamW([c, a, b]).step()
+    whole = torch.zeros(600, device="cuda")  # (side by side is no overlap)
+    halves = [torch.nn.Parameter(whole[:300]), torch.nn.Parameter(whole[300:])]
+    for p in halves:
+        p.grad = torch.ones_like(p)
+    G.FusedAdamW(halves, lr=0.5, weight_decay=0.0).step()
+    # the first step is -lr g / (|g| + eps): the root, the reciprocal and the corrections are off by a few units of 2^-24 each
+    assert torch.allclose(whole, torch.full_like(whole, -0.5), rtol=1e-6, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_whose_memory_moved(bits):
+    """A state tensor whose data lie elsewhere since the last step is read and written where it is now."""
+    def run(move):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 700, device="cuda"))
+        opt = G.FusedAdamW([p], lr=1e-2, state_bits=bits)
+        for k in range(4):
+            p.grad = torch.linspace(1, 2, 700, device="cuda") * (k + 1)
+            opt.step()
+            if move:
+                for v in opt.state[p].values():
+                    old = v.data
+                    v.data = old.clone()
+                    (old if old.element_size() > 1 else old.view(torch.uint8)).zero_()
+        return p.detach()
+
+    assert torch.equal(run(False), run(True))
