@@ -490,12 +490,15 @@ extern "C" int gcpnet_block_norm_forward(const gcp_block_norm_t* n, void* s, voi
     a.s = s; a.h = h; a.stats = stats;
     return by_type(n->type, [&](auto e) {
         typedef decltype(e) E;
+        bool fits = true;  // (a launch has less than 2^32 threads)
         const bool ok = by_shape<E>(n->d, [&](auto g, auto nv) {
             constexpr int G = g.value, T = G > 256 ? G : 256;
             const int64_t blocks = (n->rows + T / G - 1) / (T / G);
+            fits = blocks * T <= UINT32_MAX;
+            if (!fits) return;
             hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<E, G, nv.value>), dim3((unsigned)blocks), dim3(T), 0, (hipStream_t)stream, a);
         });
-        if (!ok) return GCPNET_E_UNSUPPORTED;
+        if (!ok || !fits) return GCPNET_E_UNSUPPORTED;
         GCP_HIP_CHECK_LAUNCH();
         return 0;
     });

@@ -106,7 +106,7 @@ __device__ __forceinline__ void elem_act_with(int act, float slope, const float 
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float x = v[j];
-            a[j] = x > 0.f || act == GCP_ACT_NONE ? x : (low == 0.f ? 0.f : low * x);
+            a[j] = x < 0.f ? (low == 0.f ? 0.f : low * x) : x;  // (NaN stays)
             if constexpr (GRAD) d[j] = x > 0.f ? 1.f : low;
         }
     }

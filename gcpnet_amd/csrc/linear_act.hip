@@ -613,11 +613,14 @@ void by_form(int form, F f) {
 #undef FORM
 }
 
+// Workgroups of one product: two products of one launch at 512 threads stay below the 2^32 that a launch can have.
+constexpr int64_t MAX_GROUPS = (1 << 22) - 1;
+
 // C[m][n] = sum_k A[m][k] B[n][k] with the epilogue; A and B in pieces, as [m][k] and [n][k] or, across, [k][m] and [k][n].
 template <class E>
 int describe(Gemm& g, int& shape, int64_t m, int64_t n, int64_t k, const Mat& a, bool a_across, const Mat& b, bool b_across, const Epilogue& e, float*& ws) {
     const GcpLinearPlan plan = gcp_linear_plan(m, n, k, (int)sizeof(typename E::type));
-    if (plan.tiles_m * plan.splits > INT32_MAX / 2 / plan.tiles_n) return GCPNET_E_UNSUPPORTED;
+    if (plan.tiles_m * plan.splits > MAX_GROUPS / plan.tiles_n) return GCPNET_E_UNSUPPORTED;
     if (plan.splits > 1 && !ws) return GCPNET_E_BADARG;
     shape = plan.shape;
     g = {};

@@ -306,6 +306,12 @@ def test_refusals():
     assert call() == 0
 
 
+def test_more_workgroups_than_a_launch_takes():
+    q = _lib.LinearDesc()
+    q.rows, q.k, q.n, q.x, q.w, q.x_ld, q.w_ld = 1 << 30, 4, 4, 4096, 4096, 4, 4
+    assert _lib.load().gcpnet_linear_act_forward(q, None, 0, 4096, None, 4096, None) == -2
+
+
 def test_every_tile_is_visited_once():
     """The order of the tiles (a model of gcp_tile_of_block) is a permutation, also where their number is no multiple of 8."""
     for tiles_m in (1, 2, 7, 8, 9, 17, 40):
@@ -333,3 +339,13 @@ def test_refusals_of_tensors():
             G.linear_act(*args)
     with pytest.raises(_lib.GcpnetHipError):
         G.linear_act(x, w.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [None, "relu", "leakyrelu", "selu", "silu", "sigmoid"])
+@pytest.mark.parametrize("rows", [5, 40])
+def test_nan_passes_every_activation(rows, act):
+    x, w, b, r, _ = make(rows, 72, 48, torch.float32)
+    x[3, 5] = math.nan
+    y = G.linear_act(x, w, b, act, residual=r)
+    assert torch.isnan(y[3]).all() and torch.isfinite(y[[i for i in range(rows) if i != 3]]).all()

@@ -369,6 +369,21 @@ def test_refusals():
     assert lib.gcpnet_block_norm_backward_scratch(n) == -1
 
 
+def test_more_threads_than_a_launch_takes():
+    n = _lib.BlockNorm()
+    n.rows, n.d, n.x, n.x_ld, n.eps, n.pre = 1 << 30, 8, 4096, 8, 1e-5, 1
+    assert _lib.load().gcpnet_block_norm_forward(n, None, 4096, None, None) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [None, "relu", "leakyrelu", "selu", "silu", "sigmoid"])
+def test_a_gate_that_is_nan_stays_in_its_row(act):
+    x, y, gate = (torch.randn(6, 32, device="cuda") for _ in range(3))
+    gate[2, 3] = math.nan
+    s, h = G.residual_norm(x, y, gate, gate_act=act, pre="rms")
+    assert torch.isnan(s[2, 3]) and torch.isnan(h[2]).all() and int(torch.isnan(s).sum()) == 1 and torch.isfinite(h[[0, 1, 3, 4, 5]]).all()
+
+
 @pytest.mark.gpu
 def test_refusals_of_tensors():
     x, w = torch.zeros(2, 8, device="cuda"), torch.ones(8, device="cuda")
