@@ -4,7 +4,8 @@
 //   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Bound: HBM.  Per element the step moves 28 B (fp32, fp32 moments), 16 B (fp32, 8-bit moments), 30 / 18 B (bf16 parameters: gradient
-// and parameter 2 B each way, master copy 4 B each way).  A wave owns 256 consecutive elements at a time, four per lane, so every
+// and parameter 2 B each way, master copy 4 B each way): 10^8 elements take 532 us in the first form (5.26 TB/s) and, bf16 with 8-bit
+// moments, 340 - 350 us (5.2 TB/s).  A wave owns 256 consecutive elements at a time, four per lane, so every
 // load and store is one contiguous piece per wave and the scale of 256 8-bit moments is one wave reduction; a workgroup owns a chunk
 // of 4096 elements, loads all of it before it computes, and finds its tensor by bisection in the launch arguments, so tensors of any
 // mixture of sizes fill the chip.

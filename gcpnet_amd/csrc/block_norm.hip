@@ -6,11 +6,14 @@
 //   dx = gs;  du = scale act(gate) gs;  dgate = scale gs u act'(gate);  dy = rstd1 (du w - mean(du w) - n1 mean(du w n1))
 //   weights and biases: column sums of dh n2, dh, du n1, du, and of dgate for a gate of one value per channel.
 //
-// Bound: HBM -- forward reads x, y (and an element-wise gate) and writes s, h; backward reads x, y, ds, dh, writes dx, dy (s is formed again
-// from x as the forward formed it, unrounded, for the same bytes that reading it would take).  A row is
-// held in the registers of a group of 8 to 1024 threads between its reductions, so everything is read once; the statistics take
-// two passes over the registers (mean, then squares of the differences).  The backward's groups walk many rows and keep the column sums
-// in registers; one partial sum per workgroup goes through memory, summed in a fixed order by a second launch.
+// Bound: HBM -- forward reads x, y (and an element-wise gate) and writes s, h; backward reads x, y, ds, dh, writes dx, dy (s is formed
+// again from x as the forward formed it, unrounded, for the same bytes that reading it would take).  A row is held in the registers of
+// a group of 8 to 1024 threads between its reductions, so everything is read once; the statistics take two passes over the registers
+// (mean, then squares of the differences).  The backward's groups walk many rows and keep the column sums in registers; one partial sum
+// per workgroup goes through memory, summed in a fixed order by a second launch.
+//
+// 16384 x 4096 bf16, an element-wise gate, RMS norms: forward 127 us (5.3 TB/s), backward 290 us (3.7 TB/s: eight streams, and two sums
+// over each row that all of its threads wait for).
 #include <type_traits>
 
 #include "elem_types.h"

@@ -11,7 +11,7 @@
 //   * a tile is two steps of the 16-bit matrix instructions; while one step's fragments are multiplied the next step's are read, B's into
 //     a second set of registers, A's into the registers of the row of products just issued; the waves meet once a tile, and the direct loads
 //     of the next free buffer are spread between the rows of products (all at once they held the matrix pipe up: 8192 x 4096 x 4096 bf16
-//     240 us, spread 223.5 = 1.23 PFLOP/s);
+//     240 us, spread 223.5 = 1.23 PFLOP/s; with SiLU, residual and z 260 us, its backward 508 us for both products);
 //   * an operand with k across memory keeps its layout in LDS, [k][m]; 16-bit fragments come out of it through the transposing LDS
 //     read, fp32 ones element by element;
 //   * operands whose rows are not whole 16-byte pieces are first copied into the workspace, rows filled up with zeros (one launch for all of
@@ -390,8 +390,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 
 static_assert(GCP_FEW_ROWS == 32, "two forms of few_rows_kernel");
 // Few rows (up to 16 MT): bound by the read of W, which goes from memory straight into the fragments of the matrix instructions, 512
-// consecutive bytes of each of 16 rows per wave and turn (4 rows, 4096 -> 8192 bf16: 14.6 us, 4.6 TB/s).  A workgroup takes 16 columns of y, its eight waves take turns along k; their sums
-// meet in LDS.  x comes from the caches.  Loads at any alignment: nothing is copied.
+// consecutive bytes of each of 16 rows per wave and turn (4 rows, 4096 -> 8192 bf16: 13.4 us, 5.0 TB/s).  A workgroup takes 16 columns of y,
+// its eight waves take turns along k; their sums meet in LDS.  x comes from the caches.  Loads at any alignment: nothing is copied.
 struct FewRows {
     int rows, k, n;
     const void *x, *w;

@@ -9,7 +9,7 @@
  *
  * Conventions
  *   - plain pointers and sizes only; all float tensors are contiguous fp32 row-major device memory,
- *     index arrays are int32 device memory;
+ *     index arrays are int32 device memory (the operators with a GCP_TYPE_* argument take bf16 and fp16 too, and row strides);
  *   - scalar features are [rows, dim]; vector features are [rows, channels, 3]; frames are [rows, 3, 3]
  *     with frame row a in {x_diff, x_cross, x_vertical} (components/__init__.py:268);
  *   - no ownership transfer; kernels are launched on the caller's `stream` (a hipStream_t) and return
@@ -603,9 +603,9 @@ int gcpnet_adamw_step(int n, const gcp_adamw_tensor_t* tensors, int type, int st
 /* ---- Linear with its epilogue, forward and backward (fp32, bf16 or fp16; sums in fp32):
  *   z = x W^T + b;  y = act(z) + residual;   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz
  * x [rows, k], w [n, k], residual [rows, n], dy [rows, n] have unit column stride and any row stride; bias [n] of bias_type (fp32 or `type`) or
- * NULL; y, z, dx, dw, db are contiguous, db of bias_type; k, n < 2^21.  z (pre-activation, for the backward) may be NULL, without an activation
- * it is not needed.  dx, dw, db may each be NULL.  workspace: gcpnet_linear_act_workspace(l, ...) floats (16-byte aligned; NULL where that is 0),
- * which go by the descriptor as it is then passed. */
+ * NULL; y, z, dx, dw, db are contiguous, db of bias_type; k, n < 2^21, and a product has less than 2^22 tiles of 64 x 64 or more.  z
+ * (pre-activation, for the backward) may be NULL, without an activation it is not needed.  dx, dw, db may each be NULL.  workspace:
+ * gcpnet_linear_act_workspace(l, ...) floats (16-byte aligned; NULL where that is 0), which go by the descriptor as it is then passed. */
 typedef struct {
     int64_t rows;
     int k, n, type, bias_type, act;
@@ -620,8 +620,9 @@ int gcpnet_linear_act_backward(const gcp_linear_t* l, const void* z, const void*
 
 /* ---- norms before and after a residual block with its gate and residual scale (fp32, bf16 or fp16 rows; everything in between in fp32):
  *   u = post(y);  s = x + scale * act(gate) * u;  h = pre(s)
- * over `rows` rows of `d` <= 16384 elements with unit column stride and row strides x_ld, y_ld, gate_ld (gate_ld 0: one value per channel).
- * y NULL: s = x (no gate, no post).  Parameters [d] of param_type: fp32 or `type`; NULL weight = 1, NULL bias = 0.  Outputs are
+ * over `rows` rows of `d` <= 16384 elements with unit column stride and row strides x_ld, y_ld, gate_ld (gate_ld 0: one value per channel);
+ * a row takes 8 to 1024 threads, and a launch less than 2^32.  y NULL: s = x (no gate, no post).  Parameters [d] of param_type: fp32 or
+ * `type`; NULL weight = 1, NULL bias = 0.  Outputs are
  * contiguous; s may be NULL, h is needed with pre.  stats [rows, 4] (16-byte aligned) is written for the backward, or NULL. */
 enum { GCP_NORM_NONE = 0, GCP_NORM_LAYER = 1, GCP_NORM_RMS = 2 };
 typedef struct {
