@@ -12,8 +12,8 @@
 // (mean, then squares of the differences).  The backward's groups walk many rows and keep the column sums in registers; one partial sum
 // per workgroup goes through memory, summed in a fixed order by a second launch.
 //
-// 16384 x 4096 bf16, an element-wise gate, RMS norms: forward 127 us (5.3 TB/s), backward 290 us (3.7 TB/s: eight streams, and two sums
-// over each row that all of its threads wait for).
+// 16384 x 4096 bf16, an element-wise gate, RMS norms: both directions 368 us for 1745 MB (4.7 TB/s, as a copy): forward 127 us, backward
+// 244 - 264 us (eight streams, and two sums over each row that all of its threads wait for).
 #include <type_traits>
 
 #include "elem_types.h"
@@ -37,7 +37,13 @@ struct NormArgs {
     void *dx, *dy, *dgate;
     float* part;  // [blocks, sets, d]
     int slot[SETS], sets;
+    int held;  // the backward keeps the parameters in LDS
 };
+typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
+
+// The waves of a workgroup meet and see each other's LDS writes.  (__syncthreads also waits for the wave's global loads and stores: for the row
+// that was requested ahead, and for s to arrive in memory.)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Sums of K values over the G threads of a group; every thread gets them.  Groups of more than a wave exchange through LDS, in two
 // buffers in turn, so that one barrier a call is enough.
@@ -52,7 +58,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float (*lds)[2][16], in
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int k = 0; k < K; ++k) lds[turn][k][wave] = v[k];
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float t = 0.f;
@@ -123,12 +129,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
     if (a.post) normalize(u, a.post, st[0], st[1]);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = (k * G + t) * V;
         float w[V], b[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; }
-        param_load<E, V>(a.post_w, c, in[k], a.w_f32, w);
-        param_load<E, V>(a.post_b, c, in[k], a.w_f32, b);
+        const int c = (k * G + t) * V;
+        if (a.post_w) param_load<E, V>(a.post_w, c, in[k], a.w_f32).unpack(a.w_f32, w);
+        if (a.post_b) param_load<E, V>(a.post_b, c, in[k], a.w_f32).unpack(a.w_f32, b);
         if (a.post)
 #pragma unroll
             for (int j = 0; j < V; ++j) u[k][j] = fmaf(u[k][j], w[j], b[j]);
@@ -152,8 +158,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
             float w[V], b[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; }
-            param_load<E, V>(a.pre_w, c, in[k], a.w_f32, w);
-            param_load<E, V>(a.pre_b, c, in[k], a.w_f32, b);
+            if (a.pre_w) param_load<E, V>(a.pre_w, c, in[k], a.w_f32).unpack(a.w_f32, w);
+            if (a.pre_b) param_load<E, V>(a.pre_b, c, in[k], a.w_f32).unpack(a.w_f32, b);
 #pragma unroll
             for (int j = 0; j < V; ++j) s[k][j] = fmaf(s[k][j], w[j], b[j]);
             if (on) elem_store<E, V>(a.h, r * a.d + c, s[k], in[k]);
@@ -165,15 +171,26 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
 // Waves per SIMD that the backward's registers leave room for; its workgroups are counted by them.
 template <class E, int G, int NV>
 constexpr int backward_waves() { return G > 512 ? 4 : NV > 1 ? 2 : E::vec == 8 ? 3 : 4; }
+template <class E, int G, int NV>
+constexpr int backward_groups() { return backward_waves<E, G, NV>() * 256 / (G > 256 ? G : 256); }  // of a CU
+// Sets of column sums in registers: all, or with the rest in LDS, where there is room for it.
+template <class E, int G, int NV>
+constexpr int backward_kept() { return (G > 256 ? G : 256) * NV * E::vec * 12 <= 98304 ? 2 : SETS; }
+// LDS of the backward, besides the parameters
+template <class E, int G, int NV>
+constexpr int backward_lds(bool bias) {
+    return 256 + (G < 256 ? 256 * NV * E::vec * 4 : 16) + (bias && backward_kept<E, G, NV>() == 2 ? 3 * NV * E::vec * 4 * (G > 256 ? G : 256) : 16);
+}
 
 // BIAS: with the sums of the biases and of a gate of one value per channel, too.  Those lie in LDS, where each thread adds to places of its
 // own: in registers they would take the room of the row that is requested ahead.
 template <class E, int G, int NV, bool BIAS>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(G > 256 ? G : 256, E::vec == 8 && NV == 1 ? 3 : 1) void norm_bwd_kernel(NormArgs a) {
     constexpr int V = E::vec;
     constexpr int PER = (G > 256 ? G : 256) / G;
     // A gate's sigmoid is kept between its two uses where two workgroups a CU leave registers for it (16384 x 4096 bf16, both
-    // directions: 407 us against 418), and formed twice where three are to fit (60000 x 1000 fp16, backward: 275 us against 286).
+    // directions: 407 us against 418), and formed twice where three are to fit (60000 x 1000 fp16, backward: 275 us against 286; three fit
+    // with 168 registers: 249 us, with 170 two do: 354).
     constexpr bool KEEP = NV > 1;
     __shared__ float lds[2][2][16];
     __shared__ float cols[PER > 1 ? 256 * NV * V : 1];
@@ -185,7 +202,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
         const int left = a.d - (k * G + t) * V;
         in[k] = left < 0 ? 0 : left < V ? left : V;
     }
-    constexpr int T = G > 256 ? G : 256, KEPT = T * NV * V * 12 <= 98304 ? 2 : SETS;  // sets in registers
+    constexpr int T = G > 256 ? G : 256, KEPT = backward_kept<E, G, NV>();
     __shared__ f32x4 more[BIAS && KEPT == 2 ? 3 * NV * (V / 4) * T : 1];
     float sum[BIAS ? KEPT : 2][NV][V];
     auto add = [&](int q, int k, const float (&v)[V]) {  // to a set of BIAS
@@ -206,6 +223,41 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[q][k][j] = 0.f;
+    // post_w, post_b, pre_w, for all rows
+    extern __shared__ u32x4v held[];
+    constexpr int WORDS = V / 4;  // 16-byte words of a vector of fp32 parameters
+    const bool wide = E::code != GCP_TYPE_F32 && a.w_f32;
+    const int set = NV * G * (wide ? WORDS : 1);
+    if (a.held) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const void* from = q == 0 ? a.post_w : q == 1 ? a.post_b : a.pre_w;
+            if (from)
+                for (int i = threadIdx.x; i < NV * G; i += T) {
+                    const Param<E, V> v = param_load<E, V>(from, i * V, a.d - i * V < V ? a.d - i * V : V, a.w_f32);
+                    held[q * set + i] = u32x4v{v.u[0], v.u[1], v.u[2], v.u[3]};
+                    if constexpr (V == 8)
+                        if (wide) held[q * set + NV * G + i] = u32x4v{v.u[4], v.u[5], v.u[6], v.u[7]};
+                }
+        }
+        __syncthreads();
+    }
+    auto param = [&](int q, int k, float (&f)[V]) {
+        const void* from = q == 0 ? a.post_w : q == 1 ? a.post_b : a.pre_w;
+        if (!from) return;
+        Param<E, V> v;
+        if (a.held) {
+            const u32x4v x = held[q * set + k * G + t];
+            u32x4v y = {0u, 0u, 0u, 0u};
+            if constexpr (V == 8)
+                if (wide) y = held[q * set + NV * G + k * G + t];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v.u[j] = j < 4 ? x[j & 3] : y[j & 3];
+        } else {
+            v = param_load<E, V>(from, (k * G + t) * V, in[k], a.w_f32);
+        }
+        v.unpack(a.w_f32, f);
+    };
     const bool channel = a.gate && a.gate_ld == 0, full = KEEP && a.d == G * NV * V;  // (full: no thread has less than its vectors)
     struct Row { Raw<E, V> x[NV], y[NV], g[NV], ds[NV], dh[NV]; f32x4 st; };
     auto request = [&](int64_t first, Row& q) {
@@ -223,12 +275,25 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
             q.dh[k] = a.dh ? elem_load<E, V>(a.dh, r * a.d + c, n) : elem_zero<E, V>();
         }
     };
+    // Waits for the row ahead at the end of a turn, before the turn's last stores: left to itself the compiler, which cannot count the loads
+    // behind the branches, waits for all of them in front of the next turn's first use, those just requested included.
+    auto arrived = [&](Row& q) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                asm volatile("" : "+v"(q.x[k].u[j]), "+v"(q.y[k].u[j]), "+v"(q.g[k].u[j]), "+v"(q.ds[k].u[j]), "+v"(q.dh[k].u[j])::"memory");
+        asm volatile("" : "+v"(q.st)::"memory");
+    };
     // (all groups of a workgroup make the same number of turns: barriers and shuffles stay in step.  AHEAD: a row is requested one turn
     // ahead, where the registers allow it)
     constexpr bool AHEAD = G <= 512;
     const int64_t step = (int64_t)gridDim.x * PER;
     Row ahead;
-    if constexpr (AHEAD) request((int64_t)blockIdx.x * PER, ahead);
+    if constexpr (AHEAD) {
+        request((int64_t)blockIdx.x * PER, ahead);
+        arrived(ahead);
+    }
     for (int64_t first = (int64_t)blockIdx.x * PER; first < a.rows; first += step) {
         const int64_t row = first + threadIdx.x / G;
         const bool on = row < a.rows;
@@ -256,14 +321,13 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
             float m[2] = {0.f, 0.f}, n2[NV][V], dn[NV][V];
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int c = (k * G + t) * V;
                 if (a.y) {  // s, as in the forward
                     float u[V], g[V], none[V], w[V], b[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; g[j] = gr[k][j]; u[j] = yr[k][j]; }
                     if (a.post) {
-                        param_load<E, V>(a.post_w, c, in[k], a.w_f32, w);
-                        param_load<E, V>(a.post_b, c, in[k], a.w_f32, b);
+                        param(0, k, w);
+                        param(1, k, b);
 #pragma unroll
                         for (int j = 0; j < V; ++j) u[j] = fmaf((u[j] - st[0]) * st[1], w[j], b[j]);
                     }
@@ -282,7 +346,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
                 float w[V], d[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) w[j] = 1.f;
-                param_load<E, V>(a.pre_w, c, in[k], a.w_f32, w);
+                param(2, k, w);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     d[j] = dhr[k][j];  // (0 outside)
@@ -305,7 +369,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
 #pragma unroll
             for (int k = 0; k < NV; ++k)
                 if (on) elem_store<E, V>(a.dx, r * a.d + (k * G + t) * V, gs[k], in[k]);
-        if (!a.y) continue;
+        if (!a.y) {
+            if constexpr (AHEAD) arrived(ahead);
+            continue;
+        }
         float m[2] = {0.f, 0.f};  // (gs becomes du)
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -313,8 +380,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
             float w[V], b[V], n[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; }
-            param_load<E, V>(a.post_w, c, in[k], a.w_f32, w);
-            param_load<E, V>(a.post_b, c, in[k], a.w_f32, b);
+            param(0, k, w);
+            param(1, k, b);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 n[j] = (yr[k][j] - st[0]) * st[1];
@@ -358,6 +425,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
                     gs[k][j] = st[1] * fmaf(-n, m1, gs[k][j] - m0);
                 }
         }
+        if constexpr (AHEAD) arrived(ahead);
         if (a.dy)
 #pragma unroll
             for (int k = 0; k < NV; ++k)
@@ -437,7 +505,7 @@ bool by_shape(int d, F f) {
 // them than CUs (the partial sums of each have to be added).
 template <class E, int G, int NV>
 int64_t backward_blocks(int64_t rows) {
-    constexpr int T = G > 256 ? G : 256, most = 256 * (backward_waves<E, G, NV>() * 256 / T);
+    constexpr int T = G > 256 ? G : 256, most = 256 * backward_groups<E, G, NV>();
     const int64_t blocks = (rows + T / G - 1) / (T / G), few = blocks < 256 ? blocks : blocks < 1024 ? 256 : blocks / 4;
     return few < most ? few : most;
 }
@@ -549,9 +617,16 @@ extern "C" int gcpnet_block_norm_backward(const gcp_block_norm_t* n, const float
             typedef decltype(e) E;
             const bool ok = by_shape<E>(n->d, [&](auto g, auto nv) {
                 constexpr int G = g.value, T = G > 256 ? G : 256;
-                blocks = backward_blocks<E, G, nv.value>(n->rows);
-                if (bias) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<E, G, nv.value, true>), dim3((unsigned)blocks), dim3(T), 0, (hipStream_t)stream, a);
-                else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<E, G, nv.value, false>), dim3((unsigned)blocks), dim3(T), 0, (hipStream_t)stream, a);
+                constexpr int NV = nv.value;
+                blocks = backward_blocks<E, G, NV>(n->rows);
+                // Parameters in LDS where the workgroups that should reside still do: a load of them in every turn would also wait for the row
+                // requested ahead (16384 x 4096 bf16, RMS norms: 295 us against 281; layer norms 287 against 260).
+                const int lds = 3 * NV * G * 16 * (E::code != GCP_TYPE_F32 && a.w_f32 ? E::vec / 4 : 1);
+                const int own = backward_lds<E, G, NV>(bias);
+                a.held = (a.post_w || a.post_b || a.pre_w) && lds <= 49152 && (own + lds) * backward_groups<E, G, NV>() <= 160 * 1024;
+                const int dynamic = a.held ? lds : 0;
+                if (bias) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<E, G, NV, true>), dim3((unsigned)blocks), dim3(T), dynamic, (hipStream_t)stream, a);
+                else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<E, G, NV, false>), dim3((unsigned)blocks), dim3(T), dynamic, (hipStream_t)stream, a);
             });
             if (!ok) return GCPNET_E_UNSUPPORTED;
             GCP_HIP_CHECK_LAUNCH();

@@ -60,22 +60,38 @@ __device__ __forceinline__ void elem_store(void* base, int64_t at, const float (
             if (j < count) ((typename E::type*)base)[at + j] = (typename E::type)f[j];
 }
 
-// `count` of V values of a parameter vector of the rows' type, or fp32 (`f32`: uniform over the launch); without one they stay as they are
+// `count` of V values of a parameter vector of the rows' type, or fp32 (`f32`: uniform over the launch), as they lie in memory: requested
+// early, unpacked where they are used.
 template <class E, int V>
-__device__ __forceinline__ void param_load(const void* base, int64_t at, int count, bool f32, float (&f)[V]) {
-    if (!base || count <= 0) return;
+struct Param {
+    unsigned u[V];
+    __device__ __forceinline__ void unpack(bool f32, float (&f)[V]) const {
+        if (E::code != GCP_TYPE_F32 && f32) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = __uint_as_float(u[j]);
+        } else {
+            const Raw<E, V> r = {{u[0], u[1], u[2], u[3]}};
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = r[j];
+        }
+    }
+};
+template <class E, int V>
+__device__ __forceinline__ Param<E, V> param_load(const void* base, int64_t at, int count, bool f32) {
+    Param<E, V> p;
     if (E::code != GCP_TYPE_F32 && f32) {
 #pragma unroll
         for (int h = 0; h < V; h += 4) {
             const Raw<ElemF32, 4> r = elem_load<ElemF32, 4>(base, at + h, count - h < 4 ? count - h : 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[h + j] = r[j];
+            for (int j = 0; j < 4; ++j) p.u[h + j] = r.u[j];
         }
     } else {
         const Raw<E, V> r = elem_load<E, V>(base, at, count);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = r[j];
+        for (int j = 0; j < V; ++j) p.u[j] = j < 4 ? r.u[j] : 0u;
     }
+    return p;
 }
 
 // The sigmoid by the hardware's reciprocal, good to a unit in the last place of fp32.

@@ -74,7 +74,7 @@ template <class E, int V>
 __device__ __forceinline__ void bias_load(const Epilogue& e, int64_t n, int count, float (&bias)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) bias[j] = 0.f;
-    param_load<E, V>(e.bias, n, count, e.bias_f32, bias);
+    if (e.bias && count > 0) param_load<E, V>(e.bias, n, count, e.bias_f32).unpack(e.bias_f32, bias);
 }
 
 // 16 bytes per lane from memory (uniform base + offset) to LDS (lane l to base + 16 l), counted by vmcnt.  In asm, because the compiler would

@@ -188,6 +188,15 @@ def test_forms(gate, gact, post, pre, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows,d", [(9000, 40), (2100, 1000), (1100, 2044), (1100, 4096), (600, 6000), (300, 16000)])
+def test_many_rows(rows, d, wt):
+    """Several rows a group, with the parameters in LDS or, where there is no room, from memory in every turn."""
+    both_ways(rows, d, torch.bfloat16, "channel", "silu", "layer", "layer", 2, wt=wt)
+    both_ways(rows, d, torch.bfloat16, "element", "sigmoid", "rms", "rms", 1, wt=wt)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_strided_rows_and_leading_dimensions(t):
     both_ways(50, 128, t, "element", "sigmoid", "rms", "rms", 1, spread=True)
