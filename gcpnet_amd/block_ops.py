@@ -258,8 +258,9 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Op
 
     x, weight, residual: one type of fp32, bf16 and fp16; bias that type or fp32; act as in `get_nonlinearity` or None; any sizes from one row and
     one column on.  Sums are fp32 (fp32 operands on the fp32 matrix instructions: no shorter terms).  Row strides are taken as they are, other
-    layouts are copied.  The backward keeps the pre-activation in x's type, and rounds its gradient to that type as an operand of the products for
-    x and weight; the bias gradient is summed unrounded.  All sums have a fixed order, so a run repeats bit for bit."""
+    layouts are copied.  The backward keeps the pre-activation in x's type (held to its range), and rounds its gradient dz to that type as an operand
+    of the products for x and weight, where it has the range of the type: in fp16 a |dz| from 65520 on is infinite, below 3e-8 zero.  The bias
+    gradient is summed unrounded.  All sums have a fixed order, so a run repeats bit for bit."""
     _check_first(x, "x")
     _check(weight, "weight", x)
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:

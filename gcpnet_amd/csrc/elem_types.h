@@ -2,9 +2,9 @@
 #pragma once
 #include "common.h"
 
-struct ElemF32 { typedef float type; static constexpr int code = GCP_TYPE_F32, vec = 4; };
-struct ElemBf16 { typedef __bf16 type; static constexpr int code = GCP_TYPE_BF16, vec = 8; };
-struct ElemF16 { typedef _Float16 type; static constexpr int code = GCP_TYPE_F16, vec = 8; };
+struct ElemF32 { typedef float type; static constexpr int code = GCP_TYPE_F32, vec = 4; static constexpr float largest = 0x1.fffffep127f; };
+struct ElemBf16 { typedef __bf16 type; static constexpr int code = GCP_TYPE_BF16, vec = 8; static constexpr float largest = 0x1.fep127f; };
+struct ElemF16 { typedef _Float16 type; static constexpr int code = GCP_TYPE_F16, vec = 8; static constexpr float largest = 65504.f; };
 
 template <class E, int V>
 struct Raw {  // V elements as they lie in memory, 16 bytes in four registers
@@ -58,6 +58,14 @@ __device__ __forceinline__ void elem_store(void* base, int64_t at, const float (
 #pragma unroll
         for (int j = 0; j < V; ++j)
             if (j < count) ((typename E::type*)base)[at + j] = (typename E::type)f[j];
+}
+
+// A finite value held to the range of the rows' type, where the conversion would make it infinite; infinities and NaN stay.
+template <class E>
+__device__ __forceinline__ float elem_in_range(float x) {
+    if constexpr (E::code == GCP_TYPE_F32) return x;
+    const float in = __builtin_amdgcn_fmed3f(x, -E::largest, E::largest);
+    return __builtin_isfinite(x) ? in : x;
 }
 
 // `count` of V values of a parameter vector of the rows' type, or fp32 (`f32`: uniform over the launch), as they lie in memory: requested

@@ -61,7 +61,13 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, 
     const int64_t at = m * N + n;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += bias[j];
-    if (e.z) elem_store<E, V>(e.z, at, v, count);
+    if (e.z) {
+        // z past the type's range: silu'(-inf) would be -inf * 0, while every activation's slope has reached its constant at the largest number
+        float z[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = elem_in_range<E>(v[j]);
+        elem_store<E, V>(e.z, at, z, count);
+    }
     float none[V];
     elem_act<V, false>(e.act, e.slope, v, v, none);
     if (e.residual)
@@ -450,7 +456,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(FewRows a) {
         for (int y = 0; y < WAVES; ++y) v += ((const float*)part[y][t])[r * 16 + c];
         if (a.e.bias) v += (E::code != GCP_TYPE_F32 && a.e.bias_f32) ? ((const float*)a.e.bias)[n] : (float)((const T*)a.e.bias)[n];
         const int64_t at = (int64_t)m * a.n + n;
-        if (a.e.z) ((T*)a.e.z)[at] = (T)v;
+        if (a.e.z) ((T*)a.e.z)[at] = (T)elem_in_range<E>(v);
         float one[1] = {v}, none[1];
         elem_act<1, false>(a.e.act, a.e.slope, one, one, none);
         if (a.e.residual) one[0] += (float)((const T*)a.e.residual)[m * a.e.r_ld + n];
