@@ -9,6 +9,7 @@ import ctypes as C
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -34,10 +35,23 @@ def _on(t: Tensor):
 def _backward(body):
     """A backward that autograd may not differentiate again: with a graph asked for, the wrapper that makes such a use raise."""
     once = once_differentiable(body)
-    return staticmethod(lambda ctx, *grads: once(ctx, *grads) if torch.is_grad_enabled() else body(ctx, *grads))
+
+    def backward(ctx, *grads):
+        _refuse_tangents(grads)
+        return once(ctx, *grads) if torch.is_grad_enabled() else body(ctx, *grads)
+
+    return staticmethod(backward)
+
+
+def _refuse_tangents(tensors) -> None:
+    """The kernels take values only: a tangent of forward mode would be lost without a word."""
+    # (the level, a global of that module, is -1 outside forward mode: nothing to look for then)
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("gcpnet_amd: linear_act and residual_norm have no forward-mode derivatives")
 
 
 def _wants_grad(tensors) -> bool:
+    _refuse_tangents(tensors)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
