@@ -106,6 +106,19 @@ __device__ __forceinline__ Param<E, V> param_load(const void* base, int64_t at, 
 __device__ __forceinline__ float elem_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 __device__ __forceinline__ bool elem_by_sigmoid(int act) { return act == GCP_ACT_SILU || act == GCP_ACT_SIGMOID; }
 
+// exp(x) - 1 for x <= 0: the difference itself from -1/2 down, where it is good to 5 half steps, and Taylor's series to x^8 (the next term is 1.1e-8
+// of the value at most) above, where the difference would lose x in the rounding of 1 + x.
+__device__ __forceinline__ float elem_expm1(float x) {
+    float p = 1.f / 40320.f;
+    p = fmaf(p, x, 1.f / 5040.f);
+    p = fmaf(p, x, 1.f / 720.f);
+    p = fmaf(p, x, 1.f / 120.f);
+    p = fmaf(p, x, 1.f / 24.f);
+    p = fmaf(p, x, 1.f / 6.f);
+    p = fmaf(p, x, 0.5f);
+    return x > -0.5f ? fmaf(x * x, p, x) : __expf(x) - 1.f;
+}
+
 // act(v), and with GRAD also act'(v), of V values; the choice is uniform and made once for all of them.  `s`: the sigmoids of v where the
 // activation is made of them (else not looked at).
 template <int V, bool GRAD>
@@ -122,7 +135,7 @@ __device__ __forceinline__ void elem_act_with(int act, float slope, const float 
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float x = v[j];
-            a[j] = gcp_act(GCP_ACT_SELU, x, slope);
+            a[j] = x > 0.f ? GCP_SELU_SCALE * x : GCP_SELU_SCALE * GCP_SELU_ALPHA * elem_expm1(x);
             if constexpr (GRAD) d[j] = gcp_act_grad(GCP_ACT_SELU, x, slope);
         }
     } else {  // (none, relu, leakyrelu: a slope on each side)

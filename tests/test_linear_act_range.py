@@ -1,11 +1,12 @@
-"""linear_act where values leave the range of their type: pre-activations beyond the largest number of the rows' type."""
+"""linear_act where values leave the range or the resolution of their type: pre-activations beyond the largest number of the rows' type, and
+SELU close to 0."""
 import pytest
 import torch
 
 import gcpnet_amd as G
 from tests.test_linear_act import EPS32, both_ways, half, make
 
-LA = 1.0507009873554805
+LA, AL = 1.0507009873554805, 1.6732632423543772
 # act'(z) far below and far above 0
 SLOPES = {None: (1.0, 1.0), "relu": (0.0, 1.0), "leakyrelu": (0.01, 1.0), "selu": (0.0, LA), "silu": (0.0, 1.0), "sigmoid": (0.0, 0.0)}
 
@@ -59,3 +60,20 @@ def test_a_large_negative_value_among_others(rows, k, n, act):
             x[3, 5] = 200.0
     out = both_ways(x, w, b, act, r, dy)
     assert all(torch.isfinite(v).all() for v in out.values())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [5, 40])
+def test_selu_close_to_zero(rows):
+    """selu(z) = la al (exp(z) - 1) below 0, to its relative precision however small z is: exp(z) - 1 to 2 units (4 half steps), the
+    constant 1, products 2, the bias-free sum of one product 1."""
+    z = -torch.logspace(-8, 1, 4 * rows).reshape(rows, 4)
+    z[0, 0] = -1e-30
+    eye = torch.eye(4, device="cuda")
+    y = G.linear_act(z.cuda(), eye, act="selu").cpu().double()
+    want = LA * AL * torch.expm1(z.double())
+    assert ((y - want).abs() <= 8 * EPS32 * want.abs()).all(), float(((y - want) / want).abs().max())
+    gate = z.reshape(-1).cuda()
+    s, _ = G.residual_norm(torch.zeros(3, 4 * rows, device="cuda"), torch.ones(3, 4 * rows, device="cuda"), gate, gate_act="selu", pre="rms")
+    want = want.reshape(-1)
+    assert ((s[1].cpu().double() - want).abs() <= 8 * EPS32 * want.abs()).all()
