@@ -244,7 +244,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's loader converts every state tensor to its parameter's type: here the moments, scales and master copies keep theirs.
-        Moments of another kind (fp32 for a group with 8 bits, or the reverse) are refused."""
+        Moments of another kind (fp32 for a group with 8 bits, or the reverse) are refused, and so are 8-bit moments that were saved in another memory
+        order than the parameter's (their scales go by it)."""
         super().load_state_dict(state_dict)
         self._parts, self._state_ids = {}, []
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -261,6 +262,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 if key == "step":
                     new[key] = torch.as_tensor(v).detach().to(device=p.device, dtype=torch.float32).reshape(()).clone()
                 elif key == "master" or key in ("exp_avg", "exp_avg_sq"):
+                    if bits == 8 and key != "master" and v.shape == p.shape and not self._same_order(v, p):
+                        raise _lib.GcpnetHipError(f"FusedAdamW: the 8-bit state {key!r} was saved in another memory order than its parameter has now "
+                                                  "(its scales go by that order): give the parameter the saved layout first")
                     new[key] = torch.empty_like(p, dtype=v.dtype, memory_format=torch.preserve_format).copy_(v) if v.shape == p.shape else v
                 else:
                     new[key] = v.detach().to(p.device).clone() if torch.is_tensor(v) else v
@@ -271,6 +275,11 @@ class FusedAdamW(torch.optim.Optimizer):
                 new["master"] = p.detach().float()
             self._check_state(p, new, bits)
             self.state[p] = new
+
+    @staticmethod
+    def _same_order(codes, p) -> bool:
+        """Whether 256 consecutive elements in memory are the same elements of both."""
+        return p.numel() <= 256 or all(a == b for a, b, n in zip(codes.stride(), p.stride(), p.shape) if n != 1)
 
     @staticmethod
     def _check_state(p, st, bits):
