@@ -238,43 +238,65 @@ class FusedAdamW(torch.optim.Optimizer):
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
         self._parts, self._state_ids = {}, []
+        states, lacking = self.__dict__.get("_fitted") or ({}, [])  # (of a load)
+        for g, more in zip(self.param_groups, lacking):
+            g.update(more)
+        self.state.update(states)
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
 
     def load_state_dict(self, state_dict):
-        """torch's loader converts every state tensor to its parameter's type: here the moments, scales and master copies keep theirs.
-        Moments of another kind (fp32 for a group with 8 bits, or the reverse) are refused, and so are 8-bit moments that were saved in another memory
-        order than the parameter's (their scales go by it)."""
-        super().load_state_dict(state_dict)
-        self._parts, self._state_ids = {}, []
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for g in self.param_groups:  # (state of groups written by torch.optim.AdamW has no such keys)
-            g.setdefault("state_bits", self.defaults["state_bits"])
-            g.setdefault("seed", self.defaults["seed"])
-        mine = [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]
-        for i, (p, bits) in zip(saved, mine):
-            st = state_dict["state"].get(i)
-            if not st:
-                continue
-            new = {}
-            for key, v in st.items():
-                if key == "step":
-                    new[key] = torch.as_tensor(v).detach().to(device=p.device, dtype=torch.float32).reshape(()).clone()
-                elif key == "master" or key in ("exp_avg", "exp_avg_sq"):
-                    if bits == 8 and key != "master" and v.shape == p.shape and not self._same_order(v, p):
-                        raise _lib.GcpnetHipError(f"FusedAdamW: the 8-bit state {key!r} was saved in another memory order than its parameter has now "
-                                                  "(its scales go by that order): give the parameter the saved layout first")
-                    new[key] = torch.empty_like(p, dtype=v.dtype, memory_format=torch.preserve_format).copy_(v) if v.shape == p.shape else v
-                else:
-                    new[key] = v.detach().to(p.device).clone() if torch.is_tensor(v) else v
-            if p.dtype == torch.bfloat16 and bits == 32:  # (torch keeps the moments of bf16 parameters in bf16)
-                for key in ("exp_avg", "exp_avg_sq"):
-                    new[key] = new[key].float() if new[key].dtype == torch.bfloat16 else new[key]
-            if p.dtype == torch.bfloat16 and "master" not in new:
-                new["master"] = p.detach().float()
-            self._check_state(p, new, bits)
-            self.state[p] = new
+        """torch's loader converts every state tensor to its parameter's type: here the moments, scales and master copies keep theirs.  Options come
+        from the saved groups, state_bits and seed too; groups that have none of these (torch.optim.AdamW's) leave a group its own.  Moments of another
+        kind than a group's state_bits (fp32 for 8, or the reverse) are refused, and so are 8-bit moments that were saved in another memory order than
+        the parameter's (their scales go by it).  A refused load changes nothing."""
+        # (behind all other hooks: what is checked is what is loaded, and nothing of this optimizer has been touched yet)
+        hook = self.register_load_state_dict_pre_hook(lambda _, saved: self.__dict__.__setitem__("_fitted", self._fit(saved)))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+            self.__dict__.pop("_fitted", None)
+
+    def _fit(self, state_dict):
+        """The states of a state_dict as this optimizer's parameters take them, and the options that its groups lack; everything checked."""
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            return {}, []  # (torch's loader refuses these)
+        lacking = [{k: own[k] for k in ("state_bits", "seed") if k not in g} for own, g in zip(self.param_groups, groups)]
+        states = {}
+        for own, g, more in zip(self.param_groups, groups, lacking):
+            options = {**g, **more}
+            self._check_options(options)
+            for p, i in zip(own["params"], g["params"]):
+                if state_dict["state"].get(i):
+                    states[p] = self._fit_state(p, state_dict["state"][i], options["state_bits"])
+        return states, lacking
+
+    @classmethod
+    def _fit_state(cls, p, st, bits):
+        new = {}
+        for key, v in st.items():
+            if key == "step":
+                new[key] = torch.as_tensor(v).detach().to(device=p.device, dtype=torch.float32).reshape(()).clone()
+            elif not torch.is_tensor(v):
+                new[key] = v
+            elif key in ("master", "exp_avg", "exp_avg_sq") and v.shape == p.shape:
+                if bits == 8 and key != "master" and not cls._same_order(v, p):
+                    raise _lib.GcpnetHipError(f"FusedAdamW: the 8-bit state {key!r} was saved in another memory order than its parameter has now "
+                                              "(its scales go by that order): give the parameter the saved layout first")
+                new[key] = torch.empty_like(p, dtype=v.dtype, memory_format=torch.preserve_format).copy_(v)
+            else:
+                new[key] = v.detach().to(p.device).clone()
+        if p.dtype == torch.bfloat16 and bits == 32:  # (torch keeps the moments of bf16 parameters in bf16)
+            for key in ("exp_avg", "exp_avg_sq"):
+                if torch.is_tensor(new.get(key)) and new[key].dtype == torch.bfloat16:
+                    new[key] = new[key].float()
+        if p.dtype == torch.bfloat16 and "master" not in new:
+            new["master"] = p.detach().float()
+        cls._check_state(p, new, bits)
+        return new
 
     @staticmethod
     def _same_order(codes, p) -> bool:

@@ -1,4 +1,4 @@
-"""FusedAdamW: which state a load takes, and which it refuses."""
+"""FusedAdamW: which state a load takes, and which it refuses, before anything has changed."""
 import copy
 
 import pytest
@@ -27,6 +27,28 @@ def values(t, scale):
     return out
 
 
+def snapshot(opt):
+    return copy.deepcopy([{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups]), {
+        p: (st, {k: (v, v.clone() if torch.is_tensor(v) else v) for k, v in st.items()}) for p, st in opt.state.items()}
+
+
+def assert_unchanged(opt, before):
+    groups, state = before
+    assert [{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups] == groups
+    assert list(opt.state) == list(state)
+    for p, (st, held) in state.items():
+        assert opt.state[p] is st and st.keys() == held.keys()
+        for k, (v, was) in held.items():
+            assert st[k] is v and (not torch.is_tensor(v) or (v.dtype == was.dtype and torch.equal(v.float(), was.float())))
+
+
+def refuses(opt, saved, error, match):
+    before = snapshot(opt)
+    with pytest.raises(error, match=match):
+        opt.load_state_dict(saved)
+    assert_unchanged(opt, before)
+
+
 # ---------------------------------------------------------------------------------------------------------------- layouts of 8-bit state
 @pytest.mark.parametrize("shape", [(40, 30), (6, 5, 4, 7), (3, 1, 300)])
 def test_codes_keep_their_scales_or_are_refused(shape):
@@ -45,8 +67,7 @@ def test_codes_keep_their_scales_or_are_refused(shape):
                 got = [values(o2.state[q][k], o2.state[q][k + "_scale"]) for k in ("exp_avg", "exp_avg_sq")]
                 assert all(torch.equal(x, y) for x, y in zip(got, want))
             else:
-                with pytest.raises(_lib.GcpnetHipError, match="memory order"):
-                    o2.load_state_dict(o1.state_dict())
+                refuses(o2, o1.state_dict(), _lib.GcpnetHipError, "memory order")
 
 
 def test_one_block_and_unit_dimensions_load_in_any_layout():
@@ -58,6 +79,64 @@ def test_one_block_and_unit_dimensions_load_in_any_layout():
         o2.load_state_dict(o1.state_dict())
         for k in ("exp_avg", "exp_avg_sq"):
             assert torch.equal(values(o1.state[p][k], o1.state[p][k + "_scale"]), values(o2.state[q][k], o2.state[q][k + "_scale"]))
+
+
+# ---------------------------------------------------------------------------------------------------------------- refused loads
+def test_a_refused_load_changes_nothing():
+    a, b = torch.nn.Parameter(torch.zeros(5, 70)), torch.nn.Parameter(torch.zeros(5, 70))
+    o1, o2 = G.FusedAdamW([a], state_bits=8, lr=0.5, seed=4), G.FusedAdamW([b], state_bits=32, lr=0.25, seed=6)
+    o1.state[a] = state8(a)
+    o2.state[b] = dict(step=torch.tensor(2.0), exp_avg=torch.randn(5, 70), exp_avg_sq=torch.rand(5, 70))
+    wrong = o1.state_dict()
+    wrong["param_groups"][0]["state_bits"] = 32  # (codes, said to be fp32 moments)
+    refuses(o2, wrong, _lib.GcpnetHipError, "state_bits=32")
+    short = o1.state_dict()
+    short["state"] = {0: dict(short["state"][0], exp_avg_scale=torch.ones(1))}
+    refuses(o2, short, _lib.GcpnetHipError, "contiguous scales")
+    other = G.FusedAdamW([torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))])
+    refuses(o2, other.state_dict(), ValueError, "size")  # (torch's own refusal: another number of parameters)
+    options = o2.state_dict()
+    options["param_groups"][0]["betas"] = (1.0, 0.9)
+    refuses(o2, options, ValueError, "betas")
+
+
+def test_the_last_parameter_refused_leaves_the_first_alone():
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in (4, 5)]
+    fresh = lambda: dict(step=torch.tensor(1.0), exp_avg=torch.ones(1), exp_avg_sq=torch.ones(1))  # noqa: E731
+    opt = G.FusedAdamW(ps)
+    saved = opt.state_dict()
+    saved["state"] = {0: dict(fresh(), exp_avg=torch.ones(4), exp_avg_sq=torch.ones(4)), 1: dict(fresh(), exp_avg=torch.ones(6), exp_avg_sq=torch.ones(6))}
+    refuses(opt, saved, _lib.GcpnetHipError, "shape")
+
+
+def test_groups_without_own_options_keep_theirs():
+    """A torch.optim.AdamW state knows neither state_bits nor seed: each group keeps its own, and fp32 moments are refused for 8 bits."""
+    ps = [torch.nn.Parameter(torch.randn(4)) for _ in range(2)]
+    theirs = torch.optim.AdamW([dict(params=ps[:1]), dict(params=ps[1:])], lr=0.1)
+    opt = G.FusedAdamW([dict(params=ps[:1], seed=9), dict(params=ps[1:], state_bits=8, seed=11)], seed=3)
+    opt.load_state_dict(theirs.state_dict())  # (no state yet: only options)
+    assert [(g["state_bits"], g["seed"], g["lr"]) for g in opt.param_groups] == [(32, 9, 0.1), (8, 11, 0.1)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    theirs.step()
+    refuses(opt, theirs.state_dict(), _lib.GcpnetHipError, "state_bits=8")
+
+
+def test_hooks_of_a_load_see_and_change_what_is_loaded():
+    p, q = torch.nn.Parameter(torch.zeros(300)), torch.nn.Parameter(torch.zeros(300))
+    o1, o2 = G.FusedAdamW([p], state_bits=8), G.FusedAdamW([q], state_bits=8)
+    o1.state[p] = state8(p)
+
+    def before(opt, saved):
+        st = {0: dict(saved["state"][0], step=torch.tensor(40.0))}
+        return dict(saved, state=st)
+
+    seen = []
+    o2.register_load_state_dict_pre_hook(before)
+    o2.register_load_state_dict_post_hook(lambda opt: seen.append(opt.state[q]["exp_avg"].dtype))
+    o2.load_state_dict(o1.state_dict())
+    assert float(o2.state[q]["step"]) == 40.0 and seen == [E4M3]
+    assert float(o1.state[p]["step"]) == 3.0
 
 
 @pytest.mark.gpu
