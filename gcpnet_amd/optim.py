@@ -193,7 +193,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     Nothing of a step depends on a host value that changes: `step` is a device tensor per parameter, and step() may be captured into a
     hipGraph (GraphedStep(step_fn, optimizer=...)) once an eager step has created the state; lr, betas, eps and weight_decay are frozen
-    into a capture.  With state_bits=32 and fp32 parameters, state_dicts interchange with torch.optim.AdamW."""
+    into a capture.  With state_bits=32 and fp32 parameters, state_dicts interchange with torch.optim.AdamW; its groups with maximize, amsgrad or
+    differentiable, and torch.optim.Adam's with a weight decay, are refused."""
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  state_bits: int = 32, max_grad_norm: Optional[float] = None, seed: int = 0):
@@ -223,6 +224,11 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"FusedAdamW: betas must lie in [0, 1), got {g['betas']}")
         if g["state_bits"] not in (8, 32):
             raise ValueError(f"FusedAdamW: state_bits is 8 or 32, got {g['state_bits']}")
+        for key in ("maximize", "amsgrad", "differentiable"):  # (a group that torch.optim.AdamW wrote has them)
+            if g.get(key):
+                raise ValueError(f"FusedAdamW: {key}=True is another update than this one")
+        if not g.get("decoupled_weight_decay", True) and g["weight_decay"]:
+            raise ValueError("FusedAdamW: weight decay is decoupled from the gradient (the group is torch.optim.Adam's, with decoupled_weight_decay=False)")
 
     @classmethod
     def _check_group(cls, g):

@@ -122,6 +122,27 @@ def test_groups_without_own_options_keep_theirs():
     refuses(opt, theirs.state_dict(), _lib.GcpnetHipError, "state_bits=8")
 
 
+@pytest.mark.parametrize("option", [dict(maximize=True), dict(amsgrad=True), dict(differentiable=True)])
+def test_state_of_another_update_is_refused(option):
+    p, q = torch.nn.Parameter(torch.randn(4)), torch.nn.Parameter(torch.randn(4))
+    theirs = torch.optim.AdamW([p], **option)
+    opt = G.FusedAdamW([q])
+    refuses(opt, theirs.state_dict(), ValueError, next(iter(option)))
+    with pytest.raises(ValueError, match=next(iter(option))):
+        G.FusedAdamW([dict(params=[q], **option)])
+    opt.param_groups[0].update(option)
+    with pytest.raises(ValueError, match=next(iter(option))):
+        opt.step()
+
+
+def test_coupled_decay_is_refused():
+    p, q = torch.nn.Parameter(torch.randn(4)), torch.nn.Parameter(torch.randn(4))
+    refuses(G.FusedAdamW([q]), torch.optim.Adam([p], weight_decay=0.1).state_dict(), ValueError, "decoupled")
+    opt = G.FusedAdamW([q])
+    opt.load_state_dict(torch.optim.Adam([p], weight_decay=0.0).state_dict())  # (without decay they are the same)
+    assert opt.param_groups[0]["weight_decay"] == 0.0
+
+
 def test_hooks_of_a_load_see_and_change_what_is_loaded():
     p, q = torch.nn.Parameter(torch.zeros(300)), torch.nn.Parameter(torch.zeros(300))
     o1, o2 = G.FusedAdamW([p], state_bits=8), G.FusedAdamW([q], state_bits=8)
