@@ -440,6 +440,7 @@ class FusedAdamW(torch.optim.Optimizer):
     @staticmethod
     def _same(part, grads) -> bool:
         if (part.where is None or list(map(_address, part.params)) != part.addresses or list(map(_numel, part.params)) != part.sizes
+                or not all(map(_contiguous, part.params))  # (turned where it lies)
                 or list(map(_numel, grads)) != part.sizes or set(map(_dtype, grads)) != {part.dtype} or not all(map(_contiguous, grads))
                 or list(map(_address, itertools.chain.from_iterable(map(dict.values, part.states)))) != part.where):
             return False

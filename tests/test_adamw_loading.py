@@ -1,4 +1,4 @@
-"""FusedAdamW: which state a load takes, and which it refuses, before anything has changed."""
+"""FusedAdamW: state that does not fit is refused before anything has changed, and tables of a step follow their parameters' layout."""
 import copy
 
 import pytest
@@ -6,6 +6,7 @@ import torch
 
 import gcpnet_amd as G
 from gcpnet_amd import _lib
+from gcpnet_amd.optim import _Part
 
 E4M3 = torch.float8_e4m3fn
 
@@ -158,6 +159,31 @@ def test_hooks_of_a_load_see_and_change_what_is_loaded():
     o2.load_state_dict(o1.state_dict())
     assert float(o2.state[q]["step"]) == 40.0 and seen == [E4M3]
     assert float(o1.state[p]["step"]) == 3.0
+
+
+# ---------------------------------------------------------------------------------------------------------------- steps
+def test_tables_go_by_the_strides():
+    """A parameter turned at its address, with a gradient of the new shape, does not match the old table."""
+    p = torch.nn.Parameter(torch.zeros(4, 6))
+    st = dict(step=torch.tensor(0.0), exp_avg=torch.zeros(4, 6), exp_avg_sq=torch.zeros(4, 6))
+    g = torch.ones(4, 6)
+    part = _Part(0, torch.float32, [(p, g, st, 0)], 32)
+    assert G.FusedAdamW._same(part, [g]) and G.FusedAdamW._same(part, [g.clone()])
+    p.data = p.data.t()
+    assert not G.FusedAdamW._same(part, [torch.ones(6, 4)])
+
+
+@pytest.mark.gpu
+def test_a_parameter_turned_between_two_steps_is_refused():
+    p = torch.nn.Parameter(torch.zeros(40, 30, device="cuda"))
+    opt = G.FusedAdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    p.grad = None
+    p.data = p.data.t()
+    p.grad = torch.ones(30, 40, device="cuda")
+    with pytest.raises(_lib.GcpnetHipError, match="shape and strides"):
+        opt.step()
 
 
 @pytest.mark.gpu
