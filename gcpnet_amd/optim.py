@@ -382,6 +382,8 @@ class FusedAdamW(torch.optim.Optimizer):
             self._state_ids = list(map(id, self.state.values()))
         if len(devices) > 1 and self.max_grad_norm is not None:
             raise _lib.GcpnetHipError("FusedAdamW: max_grad_norm with parameters on several devices is not supported")
+        if not devices and self.max_grad_norm is not None:  # (no gradient: not the norm of the step before)
+            self.grad_norm = next((torch.zeros((), device=p.device) for g in self.param_groups for p in g["params"]), None)
         for dev, parts in devices.items():
             with torch.cuda.device(dev):
                 self._step_device(lib, dev, parts)

@@ -186,6 +186,26 @@ def test_a_parameter_turned_between_two_steps_is_refused():
         opt.step()
 
 
+def test_the_norm_of_no_gradients_is_zero():
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = G.FusedAdamW([p], max_grad_norm=1.0)
+    opt.grad_norm = torch.tensor(7.0)  # (of a step before)
+    opt.step()
+    assert float(opt.grad_norm) == 0.0
+
+
+@pytest.mark.gpu
+def test_a_step_without_gradients_leaves_no_old_norm():
+    p = torch.nn.Parameter(torch.zeros(4, device="cuda"))
+    opt = G.FusedAdamW([p], max_grad_norm=1.0)
+    p.grad = torch.full_like(p, 2.0)
+    opt.step()
+    assert abs(float(opt.grad_norm) - 4.0) < 1e-6
+    p.grad = None
+    opt.step()
+    assert float(opt.grad_norm) == 0.0 and opt.grad_norm.device == p.device
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
