@@ -38,7 +38,7 @@ struct NormArgs {
     float* part;  // [blocks, sets, d]
     int slot[SETS], sets;
     int held;  // the backward keeps the parameters in LDS
-    int once;  // the forward's rows begin at 16 bytes
+    int once, once_x, once_y;  // the forward's rows begin at 16 bytes; those of x and y are rows of their own
 };
 typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
 
@@ -73,6 +73,8 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float (*lds)[2][16], in
 
 // Rows that are read once, past the caches, where the parameters then stay (`once`: 16384 x 4096 bf16, an element-wise gate 132 - 136 us against 139,
 // a norm alone 84 against 94).  Not where rows begin off 16 bytes: a cache line is then asked for more than once (30000 x 1001: 66 us against 58).
+// Nor one row that stands for all of them (x or y expanded): every group reads it again (16384 x 4096 bf16 84 us against 86, 16384 x 2048 fp32 64
+// against 69).
 template <class E, int V>
 __device__ __forceinline__ Raw<E, V> row_load(const void* base, int64_t at, int count, bool once) {
     if (count == V && once) {
@@ -103,8 +105,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = (k * G + t) * V;
-        xr[k] = row_load<E, V>(a.x, r * a.x_ld + c, in[k], a.once);
-        if (a.y) yr[k] = row_load<E, V>(a.y, r * a.y_ld + c, in[k], a.once);
+        xr[k] = row_load<E, V>(a.x, r * a.x_ld + c, in[k], a.once_x);
+        if (a.y) yr[k] = row_load<E, V>(a.y, r * a.y_ld + c, in[k], a.once_y);
         else yr[k] = elem_zero<E, V>();
         if (a.gate) gr[k] = row_load<E, V>(a.gate, r * a.gate_ld + c, in[k], a.once && a.gate_ld);
     }
@@ -574,6 +576,7 @@ extern "C" int gcpnet_block_norm_forward(const gcp_block_norm_t* n, void* s, voi
     const int piece = 16 / elem_bytes(n->type);
     auto whole = [&](const void* p, int64_t ld) { return !p || (aligned16(p) && ld % piece == 0); };
     a.once = whole(n->x, n->x_ld) && whole(n->y, n->y_ld) && whole(n->gate, n->gate_ld);
+    a.once_x = a.once && n->x_ld; a.once_y = a.once && n->y_ld;  // (a row for all of them is read again)
     return by_type(n->type, [&](auto e) {
         typedef decltype(e) E;
         bool fits = true;  // (a launch has less than 2^32 threads)
