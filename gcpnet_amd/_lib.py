@@ -85,8 +85,7 @@ class AdamTensor(C.Structure):
 
 class AdamWTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p),
-                ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("step", C.c_void_p), ("n", C.c_int64), ("ordinal", C.c_uint32),
-                ("vec", C.c_int)]
+                ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("step", C.c_void_p), ("n", C.c_int64), ("ordinal", C.c_uint32)]
 
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2

@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs<BF16, EIGHT> a) {
     gcp_adamw_tensor_t T;
     T.param = slot.param; T.grad = slot.grad; T.exp_avg = slot.exp_avg; T.exp_avg_sq = slot.exp_avg_sq;
     T.n = slot.n_vec >> 1;
-    T.vec = (int)(slot.n_vec & 1);
+    const bool vec = slot.n_vec & 1;
     if constexpr (BF16) T.master = slot.master;
     if constexpr (EIGHT) { T.exp_avg_scale = slot.exp_avg_scale; T.exp_avg_sq_scale = slot.exp_avg_sq_scale; }
     const int64_t at = (int64_t)((int)blockIdx.x - a.first[lo]) * CHUNK;
@@ -307,13 +307,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs<BF16, EIGHT> a) {
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {  // (uniform over a wave: a whole piece, the end of the tensor, or nothing)
         const int64_t b = at + (k * 4 + wave) * QBLOCK;
-        if (T.vec && b + QBLOCK <= T.n) piece_load<BF16, EIGHT, true>(T, b + 4 * lane, q[k]);
+        if (vec && b + QBLOCK <= T.n) piece_load<BF16, EIGHT, true>(T, b + 4 * lane, q[k]);
         else if (b < T.n) piece_load<BF16, EIGHT, false>(T, b + 4 * lane, q[k]);
     }
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
         const int64_t b = at + (k * 4 + wave) * QBLOCK;
-        if (T.vec && b + QBLOCK <= T.n) piece_update<BF16, EIGHT, true>(a, T, b + 4 * lane, q[k], clip, lr1, root2, key);
+        if (vec && b + QBLOCK <= T.n) piece_update<BF16, EIGHT, true>(a, T, b + 4 * lane, q[k], clip, lr1, root2, key);
         else if (b < T.n) piece_update<BF16, EIGHT, false>(a, T, b + 4 * lane, q[k], clip, lr1, root2, key);
     }
 }

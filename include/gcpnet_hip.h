@@ -587,7 +587,6 @@ typedef struct {
     float* step;             /* steps taken so far, advanced by gcpnet_adamw_begin */
     int64_t n;
     uint32_t ordinal;
-    int vec;                 /* the library's own */
 } gcp_adamw_tensor_t;
 /* floats that gcpnet_grad_norm writes: sums of squares over 16384 elements each */
 int64_t gcpnet_grad_norm_partials(int n, const gcp_adamw_tensor_t* tensors);
