@@ -46,6 +46,8 @@ struct StepArgs {
 };
 static_assert(sizeof(StepArgs<false, false>) <= 4096 && sizeof(StepArgs<true, true>) <= 4096, "kernel arguments");
 
+// A bijection of 32 bits whose output bits depend evenly on the input bits: two rounds of xor-shift and multiply, with the constants that
+// C. Wellons published for it (a search for the least bias, 2018).
 __device__ __forceinline__ unsigned mix32(unsigned h) {
     h ^= h >> 16;
     h *= 0x7feb352du;

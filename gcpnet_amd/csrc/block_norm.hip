@@ -12,8 +12,8 @@
 // (mean, then squares of the differences).  The backward's groups walk many rows and keep the column sums in registers; one partial sum
 // per workgroup goes through memory, summed in a fixed order by a second launch.
 //
-// 16384 x 4096 bf16, an element-wise gate, RMS norms: both directions 368 us for 1745 MB (4.7 TB/s, as a copy): forward 124 us, backward
-// 244 - 264 us (eight streams, and two sums over each row that all of its threads wait for).
+// 16384 x 4096 bf16, an element-wise gate, RMS norms: both directions 367 us for 1745 MB (4.7 TB/s, as a copy).  Its kernels, the median of 24:
+// forward 123 us, backward 256 us (eight streams, and two sums over each row that all of its threads wait for); a norm alone 58 us.
 #include <type_traits>
 
 #include "elem_types.h"
@@ -71,8 +71,8 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float (*lds)[2][16], in
     }
 }
 
-// Rows that are read once, past the caches, where the parameters then stay (`once`: 16384 x 4096 bf16, an element-wise gate 132 - 136 us against 139,
-// a norm alone 84 against 94).  Not where rows begin off 16 bytes: a cache line is then asked for more than once (30000 x 1001: 66 us against 58).
+// Rows that are read once, past the caches, where the parameters then stay (`once`, with an element-wise gate: 16384 x 4096 bf16 127 us a call against
+// 138, 60000 x 1000 fp16 106 against 113, 16384 x 2048 fp32 106 against 125; a norm alone is at the rate of memory either way).  Not where rows begin off 16 bytes: a cache line is then asked for more than once (30000 x 1001: 66 us against 58).
 // Nor one row that stands for all of them (x or y expanded): every group reads it again (16384 x 4096 bf16 84 us against 86, 16384 x 2048 fp32 64
 // against 69).
 template <class E, int V>
@@ -504,8 +504,8 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(ColArgs a) {
 }
 
 // Group size and vectors per thread for a row of d elements: the smallest group that holds the row in one vector per thread, up to 256
-// threads, then two vectors (16384 x 4096 bf16, an element-wise gate: forward 135 us with 256 threads of two vectors against 167 with 512
-// of one, backward 271 against 325).
+// threads, then two vectors (16384 x 4096 bf16, an element-wise gate, both forms in one run of an earlier state: forward 135 us with 256 threads
+// of two vectors against 167 with 512 of one, backward 271 against 325).
 template <class E, class F>
 bool by_shape(int d, F f) {
     constexpr int V = E::vec;
