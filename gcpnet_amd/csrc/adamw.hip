@@ -22,6 +22,7 @@ typedef float f32x2v __attribute__((ext_vector_type(2)));
 
 constexpr int CHUNK = 4096, QBLOCK = 256, ITER = CHUNK / (4 * QBLOCK);  // four waves x ITER blocks of 256
 constexpr int NORM_CHUNK = 16384;
+constexpr int64_t MAX_CHUNKS = (1 << 24) - 1;  // workgroups of 256 threads in a launch, which has less than 2^32 of them
 constexpr int MAX_BEGIN = 448, MAX_NORM = 200;  // tensors per launch of the kernels before the update
 
 // A tensor as the update takes it: no more than its kind needs, so that a launch takes as many as its arguments hold.
@@ -419,8 +420,8 @@ int launch_steps(int n, const gcp_adamw_tensor_t* t, const Options& o, const flo
         int64_t c = 0;
         for (; k < n && a.n < a.MOST; ++k) {
             const int64_t more = (t[k].n + CHUNK - 1) / CHUNK;
-            if (more > INT32_MAX / 2) return GCPNET_E_UNSUPPORTED;
-            if (c + more > INT32_MAX / 2) break;
+            if (more > MAX_CHUNKS) return GCPNET_E_UNSUPPORTED;
+            if (c + more > MAX_CHUNKS) break;
             Slot<BF16, EIGHT>& s = a.t[a.n];
             s.param = t[k].param; s.grad = t[k].grad; s.exp_avg = t[k].exp_avg; s.exp_avg_sq = t[k].exp_avg_sq;
             const unsigned w = BF16 ? 8 : 16, q = EIGHT ? 4 : 16;
@@ -469,8 +470,8 @@ extern "C" int gcpnet_grad_norm(int n, const gcp_adamw_tensor_t* t, int type, fl
         for (; k < n && a.count < MAX_NORM; ++k) {
             if (t[k].n == 0) continue;
             const int64_t more = (t[k].n + NORM_CHUNK - 1) / NORM_CHUNK;
-            if (more > INT32_MAX / 2) return GCPNET_E_UNSUPPORTED;
-            if (c + more > INT32_MAX / 2) break;
+            if (more > MAX_CHUNKS) return GCPNET_E_UNSUPPORTED;
+            if (c + more > MAX_CHUNKS) break;
             a.grad[a.count] = t[k].grad;
             a.n[a.count] = t[k].n;
             a.first[a.count++] = (int)c;

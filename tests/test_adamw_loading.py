@@ -186,6 +186,18 @@ def test_a_parameter_turned_between_two_steps_is_refused():
         opt.step()
 
 
+def test_a_tensor_of_more_workgroups_than_a_launch_takes():
+    """2^24 workgroups of 256 threads are 2^32: refused on the host, for the update (4096 elements each) and for the norm (16384)."""
+    lib = _lib.load()
+    arr = (_lib.AdamWTensor * 1)()
+    for name in ("param", "grad", "exp_avg", "exp_avg_sq", "step"):
+        setattr(arr[0], name, 4096)
+    arr[0].n = 4096 * ((1 << 24) - 1) + 1
+    assert lib.gcpnet_adamw_step(1, arr, 0, 32, 1e-3, 0.9, 0.999, 1e-8, 0.0, 4096, None, 0, None) == -2
+    arr[0].n = 16384 * ((1 << 24) - 1) + 1
+    assert lib.gcpnet_grad_norm(1, arr, 0, 4096, None) == -2
+
+
 def test_the_norm_of_no_gradients_is_zero():
     p = torch.nn.Parameter(torch.zeros(4))
     opt = G.FusedAdamW([p], max_grad_norm=1.0)
