@@ -130,9 +130,9 @@ __device__ __forceinline__ void elem_act_with(int act, float slope, const float 
     } else if (act == GCP_ACT_SELU) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            // (without branches: the sides of 0 are added, one of them 0; a NaN is taken for the lower)
-            const float x = v[j], low = x > 0.f ? 0.f : x, e = __expf(low);
-            a[j] = fmaf(GCP_SELU_SCALE * GCP_SELU_ALPHA, elem_expm1(low, e), GCP_SELU_SCALE * fmaxf(x, 0.f));
+            // (both sides of 0, and one of them taken: no branches; a NaN is on the lower)
+            const float x = v[j], e = __expf(x), em = elem_expm1(x, e);
+            a[j] = (x > 0.f ? GCP_SELU_SCALE : GCP_SELU_SCALE * GCP_SELU_ALPHA) * (x > 0.f ? x : em);
             if constexpr (GRAD) d[j] = x > 0.f ? GCP_SELU_SCALE : GCP_SELU_SCALE * GCP_SELU_ALPHA * e;
         }
     } else {  // (none, relu, leakyrelu: a slope on each side)

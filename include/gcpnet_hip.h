@@ -603,7 +603,7 @@ int gcpnet_adamw_step(int n, const gcp_adamw_tensor_t* tensors, int type, int st
  *   z = x W^T + b;  y = act(z) + residual;   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz
  * x [rows, k], w [n, k], residual [rows, n], dy [rows, n] have unit column stride and any row stride; bias [n] of bias_type (fp32 or `type`) or
  * NULL; y, z, dx, dw, db are contiguous, db of bias_type; k, n < 2^21, and a product has less than 2^22 tiles of 64 x 64 or more.  z
- * (pre-activation, for the backward) may be NULL, without an activation it is not needed.  dx, dw, db may each be NULL.  workspace:
+ * (pre-activation, for the backward, held to the finite range of its type) may be NULL, without an activation it is not needed.  dx, dw, db may each be NULL.  workspace:
  * gcpnet_linear_act_workspace(l, ...) floats (16-byte aligned; NULL where that is 0), which go by the descriptor as it is then passed. */
 typedef struct {
     int64_t rows;
