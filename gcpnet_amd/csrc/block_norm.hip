@@ -12,8 +12,8 @@
 // (mean, then squares of the differences).  The backward's groups walk many rows and keep the column sums in registers; one partial sum
 // per workgroup goes through memory, summed in a fixed order by a second launch.
 //
-// 16384 x 4096 bf16, an element-wise gate, RMS norms: both directions 367 us for 1745 MB (4.7 TB/s, as a copy).  Its kernels, the median of 24:
-// forward 123 us, backward 256 us (eight streams, and two sums over each row that all of its threads wait for); a norm alone 58 us.
+// 16384 x 4096 bf16, an element-wise gate, RMS norms: both directions 367 us for 1745 MB (4.7 TB/s, as a copy).  Its kernels, the median of 24
+// in two runs: forward 123 - 125 us, backward 256 - 264 us (eight streams, and two sums over each row that all of its threads wait for); a norm alone 58 us.
 #include <type_traits>
 
 #include "elem_types.h"

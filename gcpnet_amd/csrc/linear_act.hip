@@ -11,7 +11,7 @@
 //   * a tile is two steps of the 16-bit matrix instructions; while one step's fragments are multiplied the next step's are read, B's into
 //     a second set of registers, A's into the registers of the row of products just issued; the waves meet once a tile, and the direct loads
 //     of the next free buffer are spread between the rows of products (all at once they held the matrix pipe up: 8192 x 4096 x 4096 bf16
-//     240 us, spread 223.5 = 1.23 PFLOP/s; in training, the median of 24 launches, 265 us with SiLU, residual and z, 241 us dx, 220 us dW);
+//     240 us, spread 223.5 = 1.23 PFLOP/s; in training, the median of 24 launches in two runs, 265 - 275 us with SiLU, residual and z, 241 - 253 us dx, 220 - 237 us dW);
 //   * an operand with k across memory keeps its layout in LDS, [k][m]; 16-bit fragments come out of it through the transposing LDS
 //     read, fp32 ones element by element;
 //   * operands whose rows are not whole 16-byte pieces are first copied into the workspace, rows filled up with zeros (one launch for all of
